@@ -157,6 +157,12 @@ _SIGNATURES = {
     "mui_channel_delta_max_tokens": (c_int, [c_int, c_int]),
     "mui_channel_delta_workspace_bytes": (ctypes.c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "mui_channel_delta": (c_int, [_P, c_int, _P, _P, c_long, _P, _P, _P, _P, _P, _P, c_int, c_int]),
+    "mui_paged_append": (c_int, [_P, c_int] + [_P, c_long, c_long] * 3 + [_P, _P, _P, _P, c_int, c_int, _P, c_long, c_int, _P, _P, _P, _P, c_int, c_int, c_float, _P] + [c_int] * 6),
+    "mui_paged_attention_scratch_bytes": (ctypes.c_size_t, [c_int] * 9),
+    "mui_paged_attention": (c_int, [_P, c_int, _P, c_long, c_long, _P, _P, _P, _P, c_int, c_int, _P, c_long, c_int, _P, _P, c_float, c_int, c_int, c_int, c_int, _P,
+                                    ctypes.c_size_t, _P] + [c_int] * 5),
+    "mui_sample_filtered_workspace_bytes": (ctypes.c_size_t, [c_int, c_int]),
+    "mui_sample_filtered": (c_int, [_P, c_int, _P, c_long, c_int, c_int, _P, _P, c_float, _P, c_int, _P, c_float, _P, c_float, _P, _P, _P, ctypes.c_size_t]),
     "mui_probe_read": (c_int, [_P, _P, ctypes.c_uint64, _P]),
     "mui_tune_lock": (c_int, []),
     "mui_tune_gemv": (c_int, [c_int, c_int]),

@@ -1338,6 +1338,53 @@ def mui_sample_advance(logits: torch.Tensor, next_ids: torch.Tensor, step: torch
     )
 
 
+def _per_row(value, name: str, rows: int, dtype: torch.dtype, like: torch.Tensor, off):
+    """(pointer, number) of a setting given as one number or as a tensor of one per row."""
+    if not isinstance(value, torch.Tensor):
+        return None, off if value is None else value
+    if value.dtype != dtype or value.numel() != rows or not value.is_contiguous() or value.device != like.device:
+        raise RuntimeError(f"{name} must be a number or a contiguous {dtype} tensor of {rows} on {like.device}")
+    return value.data_ptr(), off
+
+
+def mui_sample_filtered(logits: torch.Tensor, random_numbers: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(token int64 [rows], probability fp32 [rows]): each row's token from a given uniform number, fp32 in [0, 1). Settings are numbers or tensors of one per row
+    (fp32; top_k int32).
+
+    Weights are exp((logit - max) / temperature), in 64 bits; tokens stand in order of falling logits, equal ones by rising index. Kept are the first top_k (0: all); of
+    those the ones in front of which less than top_p of their weight lies (1: all); of those the ones with at least min_p times the largest weight (0: all); the
+    first one always. Drawn is the first whose cumulative weight exceeds the random number times the kept weight; probability is its share of that weight. A
+    temperature of 0 takes the largest logit. NaN and -inf are never drawn; a row of nothing else gives token 0 with probability 0."""
+    _check_cuda(logits, "logits")
+    code = _dtype_code(logits)
+    if logits.stride(-1) != 1:
+        logits = logits.contiguous()
+    v = logits.shape[-1]
+    l2 = logits if logits.dim() == 2 else logits.reshape(-1, v)
+    rows = l2.shape[0]
+    if random_numbers.dtype != torch.float32 or random_numbers.numel() != rows or not random_numbers.is_contiguous() or random_numbers.device != logits.device:
+        raise RuntimeError(f"random_numbers must be a contiguous float32 tensor of {rows} on {logits.device}")
+    ts, t = _per_row(temperature, "temperature", rows, torch.float32, l2, 1.0)
+    ks, k = _per_row(top_k, "top_k", rows, torch.int32, l2, 0)
+    ps, p = _per_row(top_p, "top_p", rows, torch.float32, l2, 1.0)
+    ms, m = _per_row(min_p, "min_p", rows, torch.float32, l2, 0.0)
+    if v < 1:
+        raise RuntimeError("logits have no vocabulary")
+    if ts is None and not t >= 0 or ps is None and not p >= 0 or ms is None and not 0 <= m <= 1 or ks is None and k < 0:
+        raise ValueError("temperature, top_k and top_p must not be negative, min_p must lie in 0 .. 1")
+    token = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    probability = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    if rows == 0:
+        return token, probability
+    lib = _lib.load()
+    nbytes = lib.mui_sample_filtered_workspace_bytes(rows, v)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+    with contextlib.nullcontext() if l2.device.index == torch.cuda.current_device() else torch.cuda.device(l2.device):
+        check(lib.mui_sample_filtered(_stream(l2), code, l2.data_ptr(), l2.stride(0) if rows > 1 else v, rows, v, random_numbers.data_ptr(), ts, t, ks, k, ps, p, ms, m,
+                                      token.data_ptr(), probability.data_ptr(), workspace.data_ptr(), nbytes), "mui_sample_filtered")
+    return token, probability
+
+
 # --------------------------------------------------------------------------------------
 # embedding (csrc/module.cpp:314-320 of the reference)
 # --------------------------------------------------------------------------------------

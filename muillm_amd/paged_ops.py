@@ -1,0 +1,190 @@
+"""Operators over a paged 8-bit key/value cache (include/muillm_amd.h, the section of that name), in the manner of muillm_ext.py: validate,
+allocate outputs with torch, hand raw pointers and the current stream to the library. Queries, keys and values are fp16 or bf16; the cache is e4m3
+with one power-of-two scale per page and KV head.
+
+A call's tokens stand one after another, those of request b in the rows offsets[b] .. offsets[b + 1] - 1 (no offsets: row b is request b's only
+one). lengths[b] counts the request's tokens with the call's among them, so paged_append and paged_attention of one step take the same table,
+lengths and offsets. All three live on the device: a captured step goes on as they change. Rows behind the last request are left as they were."""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import MUI_DTYPE_BF16, MUI_DTYPE_F16, check
+
+PAGE_TOKENS = (64, 128, 256)
+HEAD_DIMS = (64, 128, 256)
+
+_CODES = {torch.float16: MUI_DTYPE_F16, torch.bfloat16: MUI_DTYPE_BF16}
+
+
+class PagedKV:
+    """One layer's pages. k: e4m3 [pages, kv_heads, page / 64, dim / 64, 64, 64], the last two token and dimension; v: e4m3 [pages, kv_heads,
+    page / 64, dim, 4, 4, 4], the last three g, t, i of token 16 t + 4 g + i; k_scale, v_scale: fp32 [pages, kv_heads], powers of two."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "kv_heads", "page", "dim", "device")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        if k.dim() != 6 or k.shape[4:] != (64, 64) or v.dim() != 7 or v.shape[4:] != (4, 4, 4):
+            raise RuntimeError("k must be [pages, kv_heads, page / 64, dim / 64, 64, 64] and v [pages, kv_heads, page / 64, dim, 4, 4, 4]")
+        self.n_pages, self.kv_heads, self.page, self.dim = k.shape[0], k.shape[1], k.shape[2] * 64, k.shape[3] * 64
+        if tuple(v.shape[:4]) != (self.n_pages, self.kv_heads, k.shape[2], self.dim):
+            raise RuntimeError(f"v has shape {tuple(v.shape)}, which does not go with k's {tuple(k.shape)}")
+        if self.page not in PAGE_TOKENS or self.dim not in HEAD_DIMS:
+            raise RuntimeError(f"pages hold {PAGE_TOKENS} tokens and heads {HEAD_DIMS} dimensions, not {self.page} and {self.dim}")
+        for name, t, dtype in (("k", k, torch.float8_e4m3fn), ("v", v, torch.float8_e4m3fn), ("k_scale", k_scale, torch.float32), ("v_scale", v_scale, torch.float32)):
+            if t.dtype != dtype or not t.is_contiguous() or t.device != k.device:
+                raise RuntimeError(f"{name} must be a contiguous {dtype} tensor on {k.device}")
+        if k_scale.shape != (self.n_pages, self.kv_heads) or v_scale.shape != k_scale.shape:
+            raise RuntimeError("k_scale and v_scale must be [pages, kv_heads]")
+        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
+
+    @classmethod
+    def empty(cls, n_pages: int, kv_heads: int, page: int, dim: int, device) -> "PagedKV":
+        """Pages of zeros."""
+        if page not in PAGE_TOKENS or dim not in HEAD_DIMS:
+            raise RuntimeError(f"pages hold {PAGE_TOKENS} tokens and heads {HEAD_DIMS} dimensions, not {page} and {dim}")
+        k, v = (torch.zeros(n_pages * kv_heads * page * dim, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2))
+        ks, vs = (torch.ones((n_pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2))
+        return cls(k.view(n_pages, kv_heads, page // 64, dim // 64, 64, 64), v.view(n_pages, kv_heads, page // 64, dim, 4, 4, 4), ks, vs)
+
+    def dense(self, pages: torch.Tensor, tokens: int):
+        """(keys, values) fp32 [kv_heads, tokens, dim] of a request whose pages these are (torch operations, for a look at the cache)."""
+        need = -(-tokens // self.page)
+        pages = pages[:need].long()
+        k = self.k.view(torch.uint8)[pages].permute(0, 1, 2, 4, 3, 5).reshape(need, self.kv_heads, self.page, self.dim)
+        v = self.v.view(torch.uint8)[pages].permute(0, 1, 2, 5, 4, 6, 3).reshape(need, self.kv_heads, self.page, self.dim)
+        return tuple((x.view(torch.float8_e4m3fn).float() * s[pages][..., None, None]).transpose(0, 1).reshape(self.kv_heads, -1, self.dim)[:, :tokens]
+                     for x, s in ((k, self.k_scale), (v, self.v_scale)))
+
+
+def _call(device: torch.device, fn, *args) -> int:
+    if device.index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
+def _rows(x: torch.Tensor, name: str, kv: PagedKV, heads: Optional[int], dtype: torch.dtype, n_rows: int):
+    """[rows, heads, dim] with whole heads: its strides between tokens and heads."""
+    if not x.is_cuda or x.device != kv.device:
+        raise RuntimeError(f"{name} must be a CUDA tensor on {kv.device}")
+    if x.dtype != dtype or x.dim() != 3 or x.shape[0] != n_rows or x.shape[2] != kv.dim or (heads is not None and x.shape[1] != heads):
+        raise RuntimeError(f"{name} has shape {tuple(x.shape)} and type {x.dtype}, expected {dtype} [{n_rows}, {heads or 'heads'}, {kv.dim}]")
+    if x.stride(2) != 1:
+        raise RuntimeError(f"{name}'s heads must be contiguous")
+    return x.stride(0), x.stride(1)
+
+
+def _places(kv: PagedKV, table: torch.Tensor, lengths: torch.Tensor, offsets: Optional[torch.Tensor], n_rows: int) -> int:
+    if not (table.is_cuda and lengths.is_cuda) or table.device != kv.device or lengths.device != kv.device:
+        raise RuntimeError(f"table and lengths must be CUDA tensors on {kv.device}")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1 or table.shape[1] < 1:
+        raise RuntimeError("table must be int32 [requests, pages] with contiguous rows")
+    n = table.shape[0]
+    if lengths.dtype != torch.int64 or lengths.shape != (n,) or not lengths.is_contiguous():
+        raise RuntimeError(f"lengths must be a contiguous int64 tensor [{n}]")
+    if offsets is None:
+        if n_rows != n:
+            raise RuntimeError(f"{n_rows} rows of {n} requests need offsets")
+    elif offsets.dtype != torch.int64 or offsets.shape != (n + 1,) or not offsets.is_contiguous() or offsets.device != kv.device:
+        raise RuntimeError(f"offsets must be a contiguous int64 tensor [{n + 1}] on {kv.device}")
+    return n
+
+
+def _dtype(x: torch.Tensor) -> int:
+    code = _CODES.get(x.dtype)
+    if code is None:
+        raise RuntimeError(f"unsupported dtype {x.dtype}: fp16 or bf16")
+    return code
+
+
+def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, kv: PagedKV, table: torch.Tensor, lengths: torch.Tensor,
+                 offsets: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                 interleaved: bool = False, rope_scale: float = 1.0, max_tokens: Optional[int] = None, out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Rotated queries [rows, heads, dim]; keys, rotated, and values go to their places in the cache. q [rows, heads, dim] (or None), k, v [rows, kv_heads,
+    dim] may be slices of one projection's output (whole heads, strides of multiples of 8, 16-byte aligned).
+
+    The first 2 * len(inv_freq) dimensions (a multiple of 16; none without inv_freq) turn by the angles position * inv_freq, fp64: as halves (i, i + n) or,
+    interleaved, as pairs (2 i, 2 i + 1); rope_scale multiplies cosine and sine (frequencies of a scaled context and their factor are the caller's). Positions
+    are the tokens' own unless positions (int64 [rows]) says otherwise.
+
+    A page's scale is the smallest power of two with which its largest value fits 448, and does not fall while earlier tokens stand there; where it
+    rises their codes follow. Infinities and NaN become NaN. A page that is appended to belongs to one request. Tokens without a place (a table entry that is no
+    page, a length beyond the table) are not written. max_tokens: at least the most new tokens of a request (default: 1 without offsets, else all rows)."""
+    n_rows = k.shape[0]
+    n = _places(kv, table, lengths, offsets, n_rows)
+    code = _dtype(k)
+    kt, kh = _rows(k, "k", kv, kv.kv_heads, k.dtype, n_rows)
+    vt, vh = _rows(v, "v", kv, kv.kv_heads, k.dtype, n_rows)
+    heads = qt = qh = 0
+    if q is not None:
+        qt, qh = _rows(q, "q", kv, None, k.dtype, n_rows)
+        heads = q.shape[1]
+        if out is None:
+            out = torch.empty((n_rows, heads, kv.dim), dtype=q.dtype, device=q.device)
+        elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or out.device != q.device:
+            raise RuntimeError("out must be a contiguous tensor of q's shape and type")
+    rot = 0
+    if inv_freq is not None:
+        rot = 2 * inv_freq.numel()
+        if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.device != kv.device:
+            raise RuntimeError(f"inv_freq must be a contiguous float64 tensor [rotated dimensions / 2] on {kv.device}")
+        if rot > kv.dim or rot % 16:
+            raise RuntimeError(f"{rot} rotated dimensions: a multiple of 16, at most {kv.dim}")
+    if positions is not None and (positions.dtype != torch.int64 or positions.shape != (n_rows,) or not positions.is_contiguous() or positions.device != kv.device):
+        raise RuntimeError(f"positions must be a contiguous int64 tensor [{n_rows}] on {kv.device}")
+    if n_rows == 0:
+        return out
+    if max_tokens is None:
+        max_tokens = 1 if offsets is None else n_rows
+    lib = _lib.load()
+    check(_call(kv.device, lib.mui_paged_append, torch.cuda.current_stream(kv.device).cuda_stream, code, None if q is None else q.data_ptr(), qt, qh, k.data_ptr(), kt,
+                kh, v.data_ptr(), vt, vh, kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.n_pages, kv.page, table.data_ptr(),
+                table.stride(0), table.shape[1], lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), None if positions is None else positions.data_ptr(),
+                None if inv_freq is None else inv_freq.data_ptr(), rot, int(interleaved), rope_scale, None if q is None else out.data_ptr(), n_rows, n, max_tokens, heads,
+                kv.kv_heads, kv.dim), "mui_paged_append")
+    return out if q is not None else None
+
+
+def paged_attention(q: torch.Tensor, kv: PagedKV, table: torch.Tensor, lengths: torch.Tensor, offsets: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                    window: int = 0, keep_first: int = 0, max_tokens: Optional[int] = None, max_length: Optional[int] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """[rows, heads, dim]: causal attention of q [rows, heads, dim] (rotated; whole heads, strides of multiples of 8) over the cache, which holds the
+    new tokens already. scale > 0: of the scores (default dim ** -0.5). window > 0: a token sees the last `window` ones, itself among them, and the first
+    keep_first of its request. A token that sees nothing gives zeros; keys on a table entry that is no page do not count.
+
+    max_tokens: as in paged_append; max_length: at least the largest of lengths (default: what a row of the table can hold). Both only size the launch."""
+    n_rows = q.shape[0]
+    n = _places(kv, table, lengths, offsets, n_rows)
+    code = _dtype(q)
+    qt, qh = _rows(q, "q", kv, None, q.dtype, n_rows)
+    heads = q.shape[1]
+    if heads == 0 or heads % kv.kv_heads:
+        raise RuntimeError(f"{heads} query heads do not go with {kv.kv_heads} key heads")
+    if window < 0 or keep_first < 0:
+        raise RuntimeError("window and keep_first must not be negative")
+    scale = kv.dim ** -0.5 if scale is None else float(scale)
+    if not scale > 0:
+        raise RuntimeError("scale must be positive")
+    if out is None:
+        out = torch.empty((n_rows, heads, kv.dim), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or out.device != q.device:
+        raise RuntimeError("out must be a contiguous tensor of q's shape and type")
+    if n_rows == 0:
+        return out
+    if max_tokens is None:
+        max_tokens = 1 if offsets is None else n_rows
+    most = min(table.shape[1] * kv.page, 0x7fffffff)
+    max_length = most if max_length is None else max(1, min(max_length, most))
+    lib = _lib.load()
+    nbytes = lib.mui_paged_attention_scratch_bytes(n_rows, n, max_tokens, max_length, window, keep_first, heads, kv.kv_heads, kv.dim)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    check(_call(kv.device, lib.mui_paged_attention, torch.cuda.current_stream(kv.device).cuda_stream, code, q.data_ptr(), qt, qh, kv.k.data_ptr(), kv.v.data_ptr(),
+                kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.n_pages, kv.page, table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
+                None if offsets is None else offsets.data_ptr(), scale, window, keep_first, max_tokens, max_length, None if scratch is None else scratch.data_ptr(), nbytes,
+                out.data_ptr(), n_rows, n, heads, kv.kv_heads, kv.dim), "mui_paged_attention")
+    return out

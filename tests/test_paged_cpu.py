@@ -1,0 +1,113 @@
+"""The paged cache and its operators without a GPU: layouts, and calls that are refused before anything runs."""
+import pytest
+import torch
+
+from muillm_amd import _lib, muillm_ext, paged_ops
+
+ARG, UNSUPPORTED, ALIGNMENT = -1, -2, -4
+P = 4096  # an aligned address that no refused call touches
+
+
+def append_args(**kw):
+    a = dict(stream=None, dtype=0, q=P, qt=512, qh=128, k=P, kt=512, kh=128, v=P, vt=512, vh=128, kp=P, vp=P, ks=P, vs=P, n_pages=4, page=64, table=P, stride=2, pages=2,
+             lengths=P, offsets=None, positions=None, inv_freq=P, rot=128, interleaved=0, factor=1.0, q_out=P, rows=2, requests=2, most=1, heads=4, kv_heads=2, dim=128)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(k=None), ARG), (dict(v=None), ARG), (dict(kp=None), ARG), (dict(vs=None), ARG), (dict(table=None), ARG), (dict(lengths=None), ARG), (dict(q_out=None), ARG),
+    (dict(n_pages=0), ARG), (dict(pages=0), ARG), (dict(stride=1), ARG), (dict(rows=0), ARG), (dict(requests=0), ARG), (dict(most=0), ARG), (dict(kv_heads=0), ARG),
+    (dict(heads=0), ARG), (dict(rot=-16), ARG), (dict(rot=144), ARG), (dict(inv_freq=None), ARG), (dict(rows=3), ARG), (dict(dtype=2), ARG), (dict(dtype=7), ARG),
+    (dict(page=32), UNSUPPORTED), (dict(page=96), UNSUPPORTED), (dict(page=512), UNSUPPORTED), (dict(dim=96, rot=64), UNSUPPORTED), (dict(rot=8), UNSUPPORTED),
+    (dict(q=P + 2), ALIGNMENT), (dict(k=P + 8), ALIGNMENT), (dict(vp=P + 4), ALIGNMENT), (dict(kt=508), ALIGNMENT), (dict(vh=132), ALIGNMENT), (dict(qt=1), ALIGNMENT),
+])
+def test_append_refusals(change, status):
+    assert _lib.load().mui_paged_append(*append_args(**change)) == status
+
+
+def attention_args(**kw):
+    a = dict(stream=None, dtype=0, q=P, qt=512, qh=128, kp=P, vp=P, ks=P, vs=P, n_pages=4, page=64, table=P, stride=2, pages=2, lengths=P, offsets=None, scale=0.1, window=0,
+             keep=0, most=1, longest=128, scratch=None, nbytes=0, out=P, rows=2, requests=2, heads=4, kv_heads=2, dim=128)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(q=None), ARG), (dict(kp=None), ARG), (dict(vp=None), ARG), (dict(ks=None), ARG), (dict(table=None), ARG), (dict(lengths=None), ARG), (dict(out=None), ARG),
+    (dict(scale=0.0), ARG), (dict(scale=-1.0), ARG), (dict(scale=float("nan")), ARG), (dict(window=-1), ARG), (dict(keep=-1), ARG), (dict(most=0), ARG),
+    (dict(longest=0), ARG), (dict(heads=5), ARG), (dict(heads=0), ARG), (dict(rows=0), ARG), (dict(rows=3), ARG), (dict(stride=1), ARG), (dict(dtype=2), ARG),
+    (dict(page=16), UNSUPPORTED), (dict(dim=192), UNSUPPORTED), (dict(requests=70000, rows=70000), UNSUPPORTED),
+    (dict(q=P + 4), ALIGNMENT), (dict(out=P + 8), ALIGNMENT), (dict(kp=P + 1), ALIGNMENT), (dict(qh=4), ALIGNMENT),
+    (dict(pages=2000, stride=2000, longest=100000), ARG),  # needs scratch and has none
+])
+def test_attention_refusals(change, status):
+    assert _lib.load().mui_paged_attention(*attention_args(**change)) == status
+
+
+def test_scratch_of_bad_sizes_is_nothing():
+    lib = _lib.load()
+    assert lib.mui_paged_attention_scratch_bytes(0, 1, 1, 100, 0, 0, 4, 2, 128) == 0
+    assert lib.mui_paged_attention_scratch_bytes(1, 1, 1, 100, 0, 0, 3, 2, 128) == 0
+    assert lib.mui_paged_attention_scratch_bytes(1, 1, 1, 0x7fffffff, 0, 0, 4, 2, 128) > 0
+
+
+def sampling_args(**kw):
+    a = dict(stream=None, dtype=0, logits=P, stride=1000, rows=2, vocab=1000, u=P, ts=None, t=1.0, ks=None, k=0, ps=None, p=1.0, ms=None, m=0.0, token=P, probability=None,
+             ws=P, nbytes=1 << 40)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(logits=None), ARG), (dict(u=None), ARG), (dict(token=None), ARG), (dict(ws=None), ARG), (dict(rows=0), ARG), (dict(vocab=0), ARG), (dict(stride=999), ARG),
+    (dict(dtype=2), ARG), (dict(nbytes=1000), ARG), (dict(rows=70000), UNSUPPORTED), (dict(vocab=0x7fffffff, stride=0x7fffffff), UNSUPPORTED), (dict(ws=P + 8), ALIGNMENT),
+])
+def test_sampling_refusals(change, status):
+    assert _lib.load().mui_sample_filtered(*sampling_args(**change)) == status
+
+
+def test_workspace_grows_with_rows_and_parts():
+    lib = _lib.load()
+    assert lib.mui_sample_filtered_workspace_bytes(0, 10) == 0 and lib.mui_sample_filtered_workspace_bytes(1, 0) == 0
+    one = lib.mui_sample_filtered_workspace_bytes(256, 1000)
+    assert one > 0 and lib.mui_sample_filtered_workspace_bytes(512, 1000) == 2 * one
+    assert lib.mui_sample_filtered_workspace_bytes(256, 200000) >= 4 * one
+
+
+def cpu_cache(page=64, dim=128, kv_heads=2, n=3):
+    return paged_ops.PagedKV.empty(n, kv_heads, page, dim, "cpu")
+
+
+def test_empty_pages_and_dense():
+    kv = cpu_cache()
+    assert (kv.n_pages, kv.kv_heads, kv.page, kv.dim) == (3, 2, 64, 128)
+    kv.k.view(torch.uint8)[1, 0, 0, 1, 5, 7] = 0x38      # 1.0: token 5, dimension 71
+    kv.v.view(torch.uint8)[1, 1, 0, 9, 2, 3, 1] = 0x40   # 2.0: token 16 * 3 + 4 * 2 + 1, dimension 9
+    kv.k_scale[1, 0], kv.v_scale[1, 1] = 0.5, 4.0
+    k, v = kv.dense(torch.tensor([2, 1], dtype=torch.int32), 128)
+    assert k.shape == v.shape == (2, 128, 128)
+    assert float(k[0, 64 + 5, 71]) == 0.5 and float(k.abs().sum()) == 0.5
+    assert float(v[1, 64 + 57, 9]) == 8.0 and float(v.abs().sum()) == 8.0
+
+
+def test_cache_refuses_other_shapes_and_types():
+    kv = cpu_cache()
+    for bad in (lambda: paged_ops.PagedKV(kv.v, kv.k, kv.k_scale, kv.v_scale), lambda: paged_ops.PagedKV(kv.k[:2], kv.v, kv.k_scale, kv.v_scale),
+                lambda: paged_ops.PagedKV(kv.k.view(torch.uint8), kv.v, kv.k_scale, kv.v_scale), lambda: paged_ops.PagedKV(kv.k, kv.v, kv.k_scale[:2], kv.v_scale),
+                lambda: paged_ops.PagedKV(kv.k, kv.v, kv.k_scale, kv.v_scale.double()), lambda: paged_ops.PagedKV.empty(2, 2, 32, 128, "cpu"),
+                lambda: paged_ops.PagedKV.empty(2, 2, 64, 96, "cpu"), lambda: paged_ops.PagedKV(kv.k[:, ::2], kv.v[:, ::2], kv.k_scale[:, ::2], kv.v_scale[:, ::2])):
+        with pytest.raises(RuntimeError):
+            bad()
+
+
+def test_tensors_of_the_cpu_are_refused():
+    kv = cpu_cache()
+    x = torch.zeros((2, 2, 128), dtype=torch.float16)
+    table, lengths = torch.zeros((2, 1), dtype=torch.int32), torch.ones(2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        paged_ops.paged_append(None, x, x, kv, table, lengths)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        paged_ops.paged_attention(x, kv, table, lengths)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        muillm_ext.mui_sample_filtered(torch.zeros((1, 10), dtype=torch.float16), torch.zeros(1))
