@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import threading
 from typing import List, Optional, Sequence, Tuple
 
@@ -33,6 +34,9 @@ from ._lib import MUI_DTYPE_BF16, MUI_DTYPE_F16, MUI_MAX_TOKENS, check
 # --------------------------------------------------------------------------------------
 # helpers
 # --------------------------------------------------------------------------------------
+_HERE = contextlib.nullcontext()  # a launch on the current device
+
+
 def _dtype_code(t: torch.Tensor) -> int:
     if t.dtype == torch.float16:
         return MUI_DTYPE_F16
@@ -1338,12 +1342,17 @@ def mui_sample_advance(logits: torch.Tensor, next_ids: torch.Tensor, step: torch
     )
 
 
-def _per_row(value, name: str, rows: int, dtype: torch.dtype, like: torch.Tensor, off):
+@functools.lru_cache(maxsize=256)
+def _sample_workspace_bytes(rows: int, vocab: int) -> int:
+    return _lib.load().mui_sample_filtered_workspace_bytes(rows, vocab)
+
+
+def _per_row(value, name: str, rows: int, dtype: torch.dtype, index: int, off):
     """(pointer, number) of a setting given as one number or as a tensor of one per row."""
     if not isinstance(value, torch.Tensor):
         return None, off if value is None else value
-    if value.dtype != dtype or value.numel() != rows or not value.is_contiguous() or value.device != like.device:
-        raise RuntimeError(f"{name} must be a number or a contiguous {dtype} tensor of {rows} on {like.device}")
+    if value.dtype is not dtype or value.numel() != rows or not value.is_contiguous() or value.get_device() != index:
+        raise RuntimeError(f"{name} must be a number or a contiguous {dtype} tensor of {rows} on the logits' device")
     return value.data_ptr(), off
 
 
@@ -1359,29 +1368,28 @@ def mui_sample_filtered(logits: torch.Tensor, random_numbers: torch.Tensor, temp
     code = _dtype_code(logits)
     if logits.stride(-1) != 1:
         logits = logits.contiguous()
-    v = logits.shape[-1]
-    l2 = logits if logits.dim() == 2 else logits.reshape(-1, v)
-    rows = l2.shape[0]
-    if random_numbers.dtype != torch.float32 or random_numbers.numel() != rows or not random_numbers.is_contiguous() or random_numbers.device != logits.device:
-        raise RuntimeError(f"random_numbers must be a contiguous float32 tensor of {rows} on {logits.device}")
-    ts, t = _per_row(temperature, "temperature", rows, torch.float32, l2, 1.0)
-    ks, k = _per_row(top_k, "top_k", rows, torch.int32, l2, 0)
-    ps, p = _per_row(top_p, "top_p", rows, torch.float32, l2, 1.0)
-    ms, m = _per_row(min_p, "min_p", rows, torch.float32, l2, 0.0)
+    v, at = logits.shape[-1], logits.get_device()
     if v < 1:
         raise RuntimeError("logits have no vocabulary")
-    if ts is None and not t >= 0 or ps is None and not p >= 0 or ms is None and not 0 <= m <= 1 or ks is None and k < 0:
+    l2 = logits if logits.dim() == 2 else logits.reshape(-1, v)
+    rows, f32 = l2.shape[0], torch.float32
+    us, _ = _per_row(random_numbers, "random_numbers", rows, f32, at, None)
+    if us is None:
+        raise RuntimeError(f"random_numbers must be a contiguous {f32} tensor of {rows}")
+    ts, t = _per_row(temperature, "temperature", rows, f32, at, 1.0)
+    ks, k = _per_row(top_k, "top_k", rows, torch.int32, at, 0)
+    ps, p = _per_row(top_p, "top_p", rows, f32, at, 1.0)
+    ms, m = _per_row(min_p, "min_p", rows, f32, at, 0.0)
+    if not t >= 0 or not p >= 0 or not 0 <= m <= 1 or k < 0:
         raise ValueError("temperature, top_k and top_p must not be negative, min_p must lie in 0 .. 1")
-    token = torch.empty(rows, dtype=torch.int64, device=logits.device)
-    probability = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    token, probability = l2.new_empty(rows, dtype=torch.int64), l2.new_empty(rows, dtype=f32)
     if rows == 0:
         return token, probability
-    lib = _lib.load()
-    nbytes = lib.mui_sample_filtered_workspace_bytes(rows, v)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
-    with contextlib.nullcontext() if l2.device.index == torch.cuda.current_device() else torch.cuda.device(l2.device):
-        check(lib.mui_sample_filtered(_stream(l2), code, l2.data_ptr(), l2.stride(0) if rows > 1 else v, rows, v, random_numbers.data_ptr(), ts, t, ks, k, ps, p, ms, m,
-                                      token.data_ptr(), probability.data_ptr(), workspace.data_ptr(), nbytes), "mui_sample_filtered")
+    nbytes = _sample_workspace_bytes(rows, v)
+    workspace = l2.new_empty(nbytes, dtype=torch.uint8)
+    with _HERE if at == torch._C._cuda_getDevice() else torch.cuda.device(at):
+        check(_lib.load().mui_sample_filtered(torch._C._cuda_getCurrentRawStream(at), code, l2.data_ptr(), l2.stride(0) if rows > 1 else v, rows, v, us, ts, t, ks, k, ps, p,
+                                              ms, m, token.data_ptr(), probability.data_ptr(), workspace.data_ptr(), nbytes), "mui_sample_filtered")
     return token, probability
 
 

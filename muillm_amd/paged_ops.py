@@ -8,6 +8,7 @@ lengths and offsets. All three live on the device: a captured step goes on as th
 
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -19,28 +20,35 @@ PAGE_TOKENS = (64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
 
 _CODES = {torch.float16: MUI_DTYPE_F16, torch.bfloat16: MUI_DTYPE_BF16}
+_E4M3, _F32, _F64, _I32, _I64 = torch.float8_e4m3fn, torch.float32, torch.float64, torch.int32, torch.int64
 
 
 class PagedKV:
     """One layer's pages. k: e4m3 [pages, kv_heads, page / 64, dim / 64, 64, 64], the last two token and dimension; v: e4m3 [pages, kv_heads,
     page / 64, dim, 4, 4, 4], the last three g, t, i of token 16 t + 4 g + i; k_scale, v_scale: fp32 [pages, kv_heads], powers of two."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "kv_heads", "page", "dim", "device")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "kv_heads", "page", "dim", "index")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
-        if k.dim() != 6 or k.shape[4:] != (64, 64) or v.dim() != 7 or v.shape[4:] != (4, 4, 4):
+        ks, vs = k.shape, v.shape
+        if len(ks) != 6 or ks[4] != 64 or ks[5] != 64 or len(vs) != 7 or vs[4] != 4 or vs[5] != 4 or vs[6] != 4:
             raise RuntimeError("k must be [pages, kv_heads, page / 64, dim / 64, 64, 64] and v [pages, kv_heads, page / 64, dim, 4, 4, 4]")
-        self.n_pages, self.kv_heads, self.page, self.dim = k.shape[0], k.shape[1], k.shape[2] * 64, k.shape[3] * 64
-        if tuple(v.shape[:4]) != (self.n_pages, self.kv_heads, k.shape[2], self.dim):
-            raise RuntimeError(f"v has shape {tuple(v.shape)}, which does not go with k's {tuple(k.shape)}")
-        if self.page not in PAGE_TOKENS or self.dim not in HEAD_DIMS:
-            raise RuntimeError(f"pages hold {PAGE_TOKENS} tokens and heads {HEAD_DIMS} dimensions, not {self.page} and {self.dim}")
-        for name, t, dtype in (("k", k, torch.float8_e4m3fn), ("v", v, torch.float8_e4m3fn), ("k_scale", k_scale, torch.float32), ("v_scale", v_scale, torch.float32)):
-            if t.dtype != dtype or not t.is_contiguous() or t.device != k.device:
+        self.n_pages, self.kv_heads, self.page, self.dim = n, h, page, dim = ks[0], ks[1], ks[2] * 64, ks[3] * 64
+        if vs[0] != n or vs[1] != h or vs[2] != ks[2] or vs[3] != dim:
+            raise RuntimeError(f"v has shape {tuple(vs)}, which does not go with k's {tuple(ks)}")
+        if page not in PAGE_TOKENS or dim not in HEAD_DIMS:
+            raise RuntimeError(f"pages hold {PAGE_TOKENS} tokens and heads {HEAD_DIMS} dimensions, not {page} and {dim}")
+        self.index = at = k.get_device()
+        for name, x, dtype in (("k", k, _E4M3), ("v", v, _E4M3), ("k_scale", k_scale, _F32), ("v_scale", v_scale, _F32)):
+            if x.dtype is not dtype or not x.is_contiguous() or x.get_device() != at:
                 raise RuntimeError(f"{name} must be a contiguous {dtype} tensor on {k.device}")
-        if k_scale.shape != (self.n_pages, self.kv_heads) or v_scale.shape != k_scale.shape:
+        if k_scale.shape != (n, h) or v_scale.shape != (n, h):
             raise RuntimeError("k_scale and v_scale must be [pages, kv_heads]")
-        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
 
     @classmethod
     def empty(cls, n_pages: int, kv_heads: int, page: int, dim: int, device) -> "PagedKV":
@@ -61,38 +69,47 @@ class PagedKV:
                      for x, s in ((k, self.k_scale), (v, self.v_scale)))
 
 
-def _call(device: torch.device, fn, *args) -> int:
-    if device.index == torch.cuda.current_device():
-        return fn(*args)
-    with torch.cuda.device(device):
-        return fn(*args)
+# (A step of small requests takes the GPU a few microseconds, so what the host does in front of it counts: the checks ask a tensor for its device's number, its
+# shape and its strides once, and the stream comes as the number that it is, not as an object.)
+def _call(index: int, fn, *args) -> int:
+    if index == torch._C._cuda_getDevice():
+        return fn(torch._C._cuda_getCurrentRawStream(index), *args)
+    with torch.cuda.device(index):
+        return fn(torch._C._cuda_getCurrentRawStream(index), *args)
 
 
 def _rows(x: torch.Tensor, name: str, kv: PagedKV, heads: Optional[int], dtype: torch.dtype, n_rows: int):
-    """[rows, heads, dim] with whole heads: its strides between tokens and heads."""
-    if not x.is_cuda or x.device != kv.device:
-        raise RuntimeError(f"{name} must be a CUDA tensor on {kv.device}")
-    if x.dtype != dtype or x.dim() != 3 or x.shape[0] != n_rows or x.shape[2] != kv.dim or (heads is not None and x.shape[1] != heads):
-        raise RuntimeError(f"{name} has shape {tuple(x.shape)} and type {x.dtype}, expected {dtype} [{n_rows}, {heads or 'heads'}, {kv.dim}]")
-    if x.stride(2) != 1:
+    """[rows, heads, dim] with whole heads: its heads and its strides between tokens and heads."""
+    s = x.shape
+    if x.get_device() != kv.index or not x.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor on the cache's device")
+    if x.dtype is not dtype or len(s) != 3 or s[0] != n_rows or s[2] != kv.dim or (heads is not None and s[1] != heads):
+        raise RuntimeError(f"{name} has shape {tuple(s)} and type {x.dtype}, expected {dtype} [{n_rows}, {heads or 'heads'}, {kv.dim}]")
+    a, b, c = x.stride()
+    if c != 1:
         raise RuntimeError(f"{name}'s heads must be contiguous")
-    return x.stride(0), x.stride(1)
+    return s[1], a, b
 
 
-def _places(kv: PagedKV, table: torch.Tensor, lengths: torch.Tensor, offsets: Optional[torch.Tensor], n_rows: int) -> int:
-    if not (table.is_cuda and lengths.is_cuda) or table.device != kv.device or lengths.device != kv.device:
-        raise RuntimeError(f"table and lengths must be CUDA tensors on {kv.device}")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1 or table.shape[1] < 1:
-        raise RuntimeError("table must be int32 [requests, pages] with contiguous rows")
-    n = table.shape[0]
-    if lengths.dtype != torch.int64 or lengths.shape != (n,) or not lengths.is_contiguous():
+def _places(kv: PagedKV, table: torch.Tensor, lengths: torch.Tensor, offsets: Optional[torch.Tensor], n_rows: int):
+    """(requests, pages of a row of the table, from row to row)"""
+    if table.get_device() != kv.index or lengths.get_device() != kv.index or not table.is_cuda:
+        raise RuntimeError("table and lengths must be CUDA tensors on the cache's device")
+    s = table.shape
+    if table.dtype is not _I32 or len(s) != 2 or s[1] < 1:
+        raise RuntimeError("table must be int32 [requests, pages]")
+    n, width = s
+    step, one = table.stride()
+    if one != 1 or (step < width and n > 1):
+        raise RuntimeError("table's rows must be contiguous")
+    if lengths.dtype is not _I64 or lengths.shape != (n,) or not lengths.is_contiguous():
         raise RuntimeError(f"lengths must be a contiguous int64 tensor [{n}]")
     if offsets is None:
         if n_rows != n:
             raise RuntimeError(f"{n_rows} rows of {n} requests need offsets")
-    elif offsets.dtype != torch.int64 or offsets.shape != (n + 1,) or not offsets.is_contiguous() or offsets.device != kv.device:
-        raise RuntimeError(f"offsets must be a contiguous int64 tensor [{n + 1}] on {kv.device}")
-    return n
+    elif offsets.dtype is not _I64 or offsets.shape != (n + 1,) or not offsets.is_contiguous() or offsets.get_device() != kv.index:
+        raise RuntimeError(f"offsets must be a contiguous int64 tensor [{n + 1}] on the cache's device")
+    return n, width, step if n > 1 else width
 
 
 def _dtype(x: torch.Tensor) -> int:
@@ -100,6 +117,19 @@ def _dtype(x: torch.Tensor) -> int:
     if code is None:
         raise RuntimeError(f"unsupported dtype {x.dtype}: fp16 or bf16")
     return code
+
+
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(*sizes: int) -> int:
+    return _lib.load().mui_paged_attention_scratch_bytes(*sizes)
+
+
+def _output(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return q.new_empty(q.shape)
+    if out.dtype is not q.dtype or out.shape != q.shape or not out.is_contiguous() or out.get_device() != q.get_device():
+        raise RuntimeError("out must be a contiguous tensor of q's shape and type")
+    return out
 
 
 def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, kv: PagedKV, table: torch.Tensor, lengths: torch.Tensor,
@@ -116,37 +146,33 @@ def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, kv
     rises their codes follow. Infinities and NaN become NaN. A page that is appended to belongs to one request. Tokens without a place (a table entry that is no
     page, a length beyond the table) are not written. max_tokens: at least the most new tokens of a request (default: 1 without offsets, else all rows)."""
     n_rows = k.shape[0]
-    n = _places(kv, table, lengths, offsets, n_rows)
-    code = _dtype(k)
-    kt, kh = _rows(k, "k", kv, kv.kv_heads, k.dtype, n_rows)
-    vt, vh = _rows(v, "v", kv, kv.kv_heads, k.dtype, n_rows)
+    n, width, step = _places(kv, table, lengths, offsets, n_rows)
+    code, dtype = _dtype(k), k.dtype
+    _, kt, kh = _rows(k, "k", kv, kv.kv_heads, dtype, n_rows)
+    _, vt, vh = _rows(v, "v", kv, kv.kv_heads, dtype, n_rows)
     heads = qt = qh = 0
+    qp = op = fp = None
     if q is not None:
-        qt, qh = _rows(q, "q", kv, None, k.dtype, n_rows)
-        heads = q.shape[1]
-        if out is None:
-            out = torch.empty((n_rows, heads, kv.dim), dtype=q.dtype, device=q.device)
-        elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or out.device != q.device:
-            raise RuntimeError("out must be a contiguous tensor of q's shape and type")
+        heads, qt, qh = _rows(q, "q", kv, None, dtype, n_rows)
+        out = _output(out, q)
+        qp, op = q.data_ptr(), out.data_ptr()
     rot = 0
     if inv_freq is not None:
-        rot = 2 * inv_freq.numel()
-        if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.device != kv.device:
-            raise RuntimeError(f"inv_freq must be a contiguous float64 tensor [rotated dimensions / 2] on {kv.device}")
+        rot, fp = 2 * inv_freq.numel(), inv_freq.data_ptr()
+        if inv_freq.dtype is not _F64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.get_device() != kv.index:
+            raise RuntimeError("inv_freq must be a contiguous float64 tensor [rotated dimensions / 2] on the cache's device")
         if rot > kv.dim or rot % 16:
             raise RuntimeError(f"{rot} rotated dimensions: a multiple of 16, at most {kv.dim}")
-    if positions is not None and (positions.dtype != torch.int64 or positions.shape != (n_rows,) or not positions.is_contiguous() or positions.device != kv.device):
-        raise RuntimeError(f"positions must be a contiguous int64 tensor [{n_rows}] on {kv.device}")
+    if positions is not None and (positions.dtype is not _I64 or positions.shape != (n_rows,) or not positions.is_contiguous() or positions.get_device() != kv.index):
+        raise RuntimeError(f"positions must be a contiguous int64 tensor [{n_rows}] on the cache's device")
     if n_rows == 0:
-        return out
+        return out if q is not None else None
     if max_tokens is None:
         max_tokens = 1 if offsets is None else n_rows
-    lib = _lib.load()
-    check(_call(kv.device, lib.mui_paged_append, torch.cuda.current_stream(kv.device).cuda_stream, code, None if q is None else q.data_ptr(), qt, qh, k.data_ptr(), kt,
-                kh, v.data_ptr(), vt, vh, kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.n_pages, kv.page, table.data_ptr(),
-                table.stride(0), table.shape[1], lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), None if positions is None else positions.data_ptr(),
-                None if inv_freq is None else inv_freq.data_ptr(), rot, int(interleaved), rope_scale, None if q is None else out.data_ptr(), n_rows, n, max_tokens, heads,
-                kv.kv_heads, kv.dim), "mui_paged_append")
+    check(_call(kv.index, _lib.load().mui_paged_append, code, qp, qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, kv.k.data_ptr(), kv.v.data_ptr(),
+                kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.n_pages, kv.page, table.data_ptr(), step, width, lengths.data_ptr(),
+                None if offsets is None else offsets.data_ptr(), None if positions is None else positions.data_ptr(), fp, rot, 1 if interleaved else 0, rope_scale, op,
+                n_rows, n, max_tokens, heads, kv.kv_heads, kv.dim), "mui_paged_append")
     return out if q is not None else None
 
 
@@ -159,32 +185,27 @@ def paged_attention(q: torch.Tensor, kv: PagedKV, table: torch.Tensor, lengths: 
 
     max_tokens: as in paged_append; max_length: at least the largest of lengths (default: what a row of the table can hold). Both only size the launch."""
     n_rows = q.shape[0]
-    n = _places(kv, table, lengths, offsets, n_rows)
+    n, width, step = _places(kv, table, lengths, offsets, n_rows)
     code = _dtype(q)
-    qt, qh = _rows(q, "q", kv, None, q.dtype, n_rows)
-    heads = q.shape[1]
+    heads, qt, qh = _rows(q, "q", kv, None, q.dtype, n_rows)
     if heads == 0 or heads % kv.kv_heads:
         raise RuntimeError(f"{heads} query heads do not go with {kv.kv_heads} key heads")
     if window < 0 or keep_first < 0:
         raise RuntimeError("window and keep_first must not be negative")
-    scale = kv.dim ** -0.5 if scale is None else float(scale)
-    if not scale > 0:
+    if scale is None:
+        scale = kv.dim ** -0.5
+    elif not scale > 0:
         raise RuntimeError("scale must be positive")
-    if out is None:
-        out = torch.empty((n_rows, heads, kv.dim), dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or out.device != q.device:
-        raise RuntimeError("out must be a contiguous tensor of q's shape and type")
+    out = _output(out, q)
     if n_rows == 0:
         return out
     if max_tokens is None:
         max_tokens = 1 if offsets is None else n_rows
-    most = min(table.shape[1] * kv.page, 0x7fffffff)
+    most = min(width * kv.page, 0x7fffffff)
     max_length = most if max_length is None else max(1, min(max_length, most))
-    lib = _lib.load()
-    nbytes = lib.mui_paged_attention_scratch_bytes(n_rows, n, max_tokens, max_length, window, keep_first, heads, kv.kv_heads, kv.dim)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    check(_call(kv.device, lib.mui_paged_attention, torch.cuda.current_stream(kv.device).cuda_stream, code, q.data_ptr(), qt, qh, kv.k.data_ptr(), kv.v.data_ptr(),
-                kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.n_pages, kv.page, table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
-                None if offsets is None else offsets.data_ptr(), scale, window, keep_first, max_tokens, max_length, None if scratch is None else scratch.data_ptr(), nbytes,
-                out.data_ptr(), n_rows, n, heads, kv.kv_heads, kv.dim), "mui_paged_attention")
+    nbytes = _scratch_bytes(n_rows, n, max_tokens, max_length, window, keep_first, heads, kv.kv_heads, kv.dim)
+    scratch = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    check(_call(kv.index, _lib.load().mui_paged_attention, code, q.data_ptr(), qt, qh, kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.n_pages,
+                kv.page, table.data_ptr(), step, width, lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), scale, window, keep_first, max_tokens, max_length,
+                None if scratch is None else scratch.data_ptr(), nbytes, out.data_ptr(), n_rows, n, heads, kv.kv_heads, kv.dim), "mui_paged_attention")
     return out
