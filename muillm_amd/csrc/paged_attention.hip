@@ -7,6 +7,8 @@
 // Sums and the running maximum are 32 bits; the maximum is rounded up to a whole power of two, so moving to a new one is exact.
 //
 // Score products are K Q^T (rows keys, columns queries), value products V^T P^T: scores leave the first as the second wants them, in registers.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace mui {
@@ -19,7 +21,8 @@ struct PagedAttnParams {
   float scale;          // of the scores, times log2(e)
   int window, keep;
   int heads, kv_heads, group;
-  int col_tiles;        // tiles of 16 columns (new token, head of the group) of a request at most
+  int block_cols;       // columns (new token, head of the group) of a workgroup
+  int col_tiles;        // such blocks of a request at most
   int split_tiles;      // tiles of 64 keys per workgroup
   int splits;           // at most
   float* part;          // [splits][n_rows * heads][dim + 2], or null: one split
@@ -107,195 +110,259 @@ __device__ __forceinline__ void load_queries(QueryTile<DC, PIECES>& t, const uin
                             u32x4{w[s][2 * m + 1][0], w[s][2 * m + 1][1], w[s][2 * m + 1][2], w[s][2 * m + 1][3]});
 }
 
-// one tile of 64 keys, as a wave holds it: 1 KB per register of 16 bytes
+// One tile of 64 keys. A chunk of 1 KB is one operand of a wave: lane (row l % 16, g) has chunk g of the row's 64 bytes.
 template <int DC>
-struct KvTile { u32x4 k[4 * DC]; u32x4 v[4 * DC]; };
-template <int DC>
-__device__ __forceinline__ void load_tile(KvTile<DC>& t, const uint8_t* k, const uint8_t* v, int lane) {
-  // lane (row l % 16, g): chunk g of row's 64 bytes
-  const int at = (lane & 15) * 64 + (lane >> 4) * 16;
+struct KvRegs {
+  u32x4 kr[4 * DC], vr[4 * DC];
+  __device__ __forceinline__ u32x4 k(int i) const { return kr[i]; }
+  __device__ __forceinline__ u32x4 v(int i) const { return vr[i]; }
+  __device__ __forceinline__ void load(const uint8_t* kp, const uint8_t* vp, int lane) {
+    const int at = (lane & 15) * 64 + (lane >> 4) * 16;
 #pragma unroll
-  for (int i = 0; i < 4 * DC; ++i) t.k[i] = ld16_stream(k + i * 1024 + at);
+    for (int i = 0; i < 4 * DC; ++i) kr[i] = ld16_stream(kp + i * 1024 + at);
 #pragma unroll
-  for (int i = 0; i < 4 * DC; ++i) t.v[i] = ld16_stream(v + i * 1024 + at);
-}
-
+    for (int i = 0; i < 4 * DC; ++i) vr[i] = ld16_stream(vp + i * 1024 + at);
+  }
+};
 // 0xff in the bytes of a dword of codes that are NaN
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   const uint32_t a = (w & 0x7f7f7f7fu) + 0x01010101u;  // 0x80 where the code is NaN
   return ((a & 0x80808080u) >> 7) * 0xffu;
 }
 
+// Which of a tile's keys first_key .. + 63 a query at `pos` sees, a bit each; from key 4 g on.
+__device__ __forceinline__ unsigned long long seen_keys(long first_key, long pos, long length, int window, int keep, int g) {
+  auto below = [](long n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; };  // keys first_key .. + n - 1
+  unsigned long long m = below((pos + 1 < length ? pos + 1 : length) - first_key);
+  if (window > 0) m &= ~below(pos - window + 1 - first_key) | below(keep - first_key);
+  return m >> (4 * g);
+}
+
+// The running result of 16 columns: lane (column, g) has dimensions 16 i + 4 g + r.
 template <int DC>
 struct Columns {
-  f32x4 o[4 * DC];  // lane (column, g), dimensions 16 i + 4 g + r
-  float m, l;       // the maximum, a whole number of powers of two; this lane's part of the sum
+  f32x4 o[4 * DC];
+  f32x4 l;  // the sum of the probabilities, as they went into the products: four times the same
+  float m;  // the maximum, a whole number of powers of two
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 4 * DC; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    l = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = kNoMax;
+  }
 };
 
-// The tile's scores and values into the running result of 16 columns. pos: the lane's column's position (-1: no column); first_key: key 0 of the tile;
+// The tile's scores and values into the results of NT times 16 columns. pos: the lane's columns' positions (-1: no column); first_key: key 0 of the tile;
 // whole: every column sees all 64 keys. `ks`, `vs`: the page's scales.
-template <typename T, int DC, int PIECES>
-__device__ __forceinline__ void attend_tile(Columns<DC>& c, const QueryTile<DC, PIECES>& q, const KvTile<DC>& t, float ks, float vs, bool whole, long first_key,
-                                            long pos, long length, int window, int keep, int g) {
+template <int DC, int PIECES, int NT, typename KV>
+__device__ __forceinline__ void attend_tile(Columns<DC> (&c)[NT], const QueryTile<DC, PIECES> (&q)[NT], const KV& kv, float ks, float vs, bool whole, long first_key,
+                                            const long (&pos)[NT], long length, int window, int keep, int g) {
   constexpr int M = (DC + 1) / 2;
   const u32x4 zero = {0, 0, 0, 0};
-  f32x4 s[4];
+  f32x4 s[NT][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      const i32x8 kk = pair8(t.k[8 * m + i], 2 * m + 1 < DC ? t.k[8 * m + 4 + i < 4 * DC ? 8 * m + 4 + i : 0] : zero);
+      const i32x8 kk = pair8(kv.k(8 * m + i), 2 * m + 1 < DC ? kv.k(2 * m + 1 < DC ? 8 * m + 4 + i : 0) : zero);
 #pragma unroll
-      for (int j = 0; j < PIECES; ++j) a = mfma_e4m3(kk, q.piece[j][m], a, 127, 127 - 5 * j);
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) s[n][i] = mfma_e4m3(kk, q[n].piece[j][m], s[n][i], 127, 127 - 5 * j);
     }
-    s[i] = a;
   }
-  const float unit = q.unit * ks;
-  uint32_t hidden = 0;  // keys 16 i + 4 g + r that the column does not see, bit 4 i + r
-  if (!whole) {
+  i32x8 pp[NT];
+  int sb[NT];
+  uint32_t seen[NT];  // keys 16 i + 4 g + r: bit 4 i + r
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (!whole) {
+      const unsigned long long m = seen_keys(first_key, pos[n], length, window, keep, g);
+      seen[n] = (uint32_t)(m & 0xf) | (uint32_t)(m >> 16 & 0xf) << 4 | (uint32_t)(m >> 32 & 0xf) << 8 | (uint32_t)(m >> 48 & 0xf) << 12;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[n][i][r] = seen[n] >> (4 * i + r) & 1u ? s[n][i][r] : -INFINITY;
+    }
+    const float unit = q[n].unit * ks;  // > 0
+    float most = s[n][0][0];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const long key = first_key + 16 * i + 4 * g + r;
-        const bool see = key <= pos && key < length && (window <= 0 || key > pos - window || key < keep);
-        hidden |= see ? 0u : 1u << (4 * i + r);
-      }
-  }
-  float most = -INFINITY;
+      for (int r = 0; r < 4; ++r) most = fmaxf(most, s[n][i][r]);
+    most = rows_max(most) * unit;
+    const float mt = fmaxf(ceilf(fminf(most, 1e30f)), kNoMax);
+    if (__any(mt > c[n].m)) {
+      const float to = fmaxf(c[n].m, mt), f = __builtin_amdgcn_exp2f(c[n].m - to);
+      c[n].m = to;
+      c[n].l *= f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (!whole && (hidden >> (4 * i + r) & 1u)) s[i][r] = -INFINITY;
-      most = fmaxf(most, s[i][r]);
+      for (int i = 0; i < 4 * DC; ++i) c[n].o[i] *= f;
     }
-  most = rows_max(most) * unit;  // (unit > 0)
-  const float mt = fmaxf(ceilf(fminf(most, 1e30f)), kNoMax);
-  if (__any(mt > c.m)) {
-    const float to = fmaxf(c.m, mt), f = __builtin_amdgcn_exp2f(c.m - to);
-    c.m = to;
-    c.l *= f;
+    // probabilities of the tile, its largest in (2^7, 2^8]
+    const float base = fabsf(mt) < 1e8f ? mt - 8.f : mt;  // (beyond, the difference would be rounded)
 #pragma unroll
-    for (int i = 0; i < 4 * DC; ++i) c.o[i] *= f;
-  }
-  // probabilities of the tile, its largest in (2^7, 2^8]
-  const float base = fabsf(mt) < 1e8f ? mt - 8.f : mt;  // (beyond, the difference would be rounded)
-  uint32_t hi[4], lo[4];
-  float sum = 0.f;
+    for (int i = 0; i < 4; ++i) {
+      float e[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float e[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      e[r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], unit, -base));
-      sum += e[r];
+      for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[n][i][r], unit, -base));
+      const uint32_t hi = to_e4m3x4(e[0], e[1], e[2], e[3]);
+      const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true);
+      pp[n][i] = (int)hi;
+      pp[n][4 + i] = (int)to_e4m3x4(e[0] - a[0], e[1] - a[1], e[2] - b[0], e[3] - b[1]);
     }
-    hi[i] = to_e4m3x4(e[0], e[1], e[2], e[3]);
-    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi[i], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi[i], true);
-    lo[i] = to_e4m3x4(e[0] - a[0], e[1] - a[1], e[2] - b[0], e[3] - b[1]);
+    sb[n] = 127 + (int)fmaxf(base - c[n].m, -127.f);
   }
-  const float up = fmaxf(base - c.m, -127.f);
-  c.l += sum * __builtin_amdgcn_exp2f(up);
-  const int sb = 127 + (int)up, sa = 127 + scale_exponent(vs);
-  const i32x8 pp = i32x8{(int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3], (int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3]};
-  if (whole) {
+  const int sa = 127 + scale_exponent(vs);
+  constexpr int kOnes = 0x38383838;
+  const i32x8 ones = {kOnes, kOnes, kOnes, kOnes, kOnes, kOnes, kOnes, kOnes};
 #pragma unroll
-    for (int i = 0; i < 4 * DC; ++i) c.o[i] = mfma_e4m3(pair8(t.v[i], t.v[i]), pp, c.o[i], sa, sb);
+  for (int n = 0; n < NT; ++n) c[n].l = mfma_e4m3(ones, pp[n], c[n].l, 127, sb[n]);
+  // Where part of the tile is hidden, what stands there may be anything, and 0 * NaN is NaN.
+  bool nan = false;
+  if (!whole) {
+    uint32_t found = 0;
+#pragma unroll
+    for (int i = 0; i < 4 * DC; ++i) {
+      const u32x4 v = kv.v(i);
+      found |= nan_bytes(v.x) | nan_bytes(v.y) | nan_bytes(v.z) | nan_bytes(v.w);
+      __builtin_amdgcn_sched_barrier(0);  // (one chunk at a time here and below: kept apart, these rare steps cost the others no registers)
+    }
+    nan = __any(found != 0);
+  }
+  if (!nan) {
+#pragma unroll
+    for (int i = 0; i < 4 * DC; ++i) {
+      const u32x4 v = kv.v(i);
+      const i32x8 vv = pair8(v, v);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) c[n].o[i] = mfma_e4m3(vv, pp[n], c[n].o[i], sa, sb[n]);
+    }
     return;
   }
-  // Part of the tile is hidden: what stands there may be anything, and 0 * NaN is NaN. A NaN code counts as zero, and a column that sees it gets a NaN.
-  uint32_t found = 0;
+  // A NaN code counts as zero, and a column that sees it gets a NaN.
 #pragma unroll
-  for (int i = 0; i < 4 * DC; ++i) {
-    u32x4 v = t.v[i];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t n = nan_bytes(v[j]);
-      found |= n;
-      v[j] &= ~n;
-    }
-    c.o[i] = mfma_e4m3(pair8(v, v), pp, c.o[i], sa, sb);
-  }
-  if (__any(found != 0)) {
-    i32x8 ones;
+  for (int n = 0; n < NT; ++n) {
+    i32x8 mine;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t w = 0;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) w |= (hidden >> (4 * i + r) & 1u) ? 0u : 0x38u << (8 * r);
-      ones[i] = (int)w;
-      ones[4 + i] = 0;
+      for (int r = 0; r < 4; ++r) w |= seen[n] >> (4 * i + r) & 1u ? 0x38u << (8 * r) : 0u;
+      mine[i] = (int)w;
+      mine[4 + i] = 0;
     }
 #pragma unroll
     for (int i = 0; i < 4 * DC; ++i) {
-      u32x4 v = t.v[i];
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4 v = kv.v(i), x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = nan_bytes(v[j]) & 0x38383838u;
-      const f32x4 seen = mfma_e4m3(pair8(v, zero), ones, f32x4{0.f, 0.f, 0.f, 0.f}, 127, 127);
+      for (int j = 0; j < 4; ++j) {
+        x[j] = nan_bytes(v[j]);
+        v[j] &= ~x[j];
+        x[j] &= 0x38383838u;
+      }
+      c[n].o[i] = mfma_e4m3(pair8(v, v), pp[n], c[n].o[i], sa, sb[n]);
+      const f32x4 sees = mfma_e4m3(pair8(x, zero), mine, f32x4{0.f, 0.f, 0.f, 0.f}, 127, 127);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (seen[r] > 0.f) c.o[i][r] = __builtin_nanf("");
+      for (int r = 0; r < 4; ++r) c[n].o[i][r] = sees[r] > 0.f ? __builtin_nanf("") : c[n].o[i][r];
     }
   }
+  __builtin_amdgcn_sched_barrier(0);
 }
 
-// Single tokens, and several: a workgroup takes 16 columns (new token, head of the group) of one KV head and `split_tiles` tiles of 64 keys, its waves
-// every fourth tile each; their results meet in LDS.
+// The columns of a block: new tokens times heads of a KV head's group, `per` from number `block * per` on.
+struct ColumnBlock {
+  int first, end;        // columns
+  long pos0, pos1;       // positions of the first and the last
+  TileRange range;
+};
+__device__ __forceinline__ ColumnBlock column_block(const PagedAttnParams& p, const PagedSpan& sp, int block, int per) {
+  ColumnBlock b;
+  const int n_cols = sp.count * p.group;  // (at most n_rows times heads, which fits)
+  b.first = block * per;
+  b.end = n_cols - b.first > per ? b.first + per : n_cols;
+  b.pos0 = sp.start + (unsigned)b.first / (unsigned)p.group;
+  b.pos1 = sp.start + (unsigned)(b.end - 1) / (unsigned)p.group;
+  b.range = tile_range(p, b.pos0, b.pos1, sp.length);
+  return b;
+}
+
+// (what a request's numbers say is the same for a workgroup, which the compiler does not see where they come from memory: in scalar registers it costs the results no room)
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long uniform(long x) {
+  return (long)((unsigned long long)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)(x & 0xffffffffL)));
+}
+__device__ __forceinline__ PagedSpan uniform(PagedSpan s) { return {uniform(s.row0), uniform(s.count), uniform(s.start), uniform(s.length)}; }
+
+// where a tile lies, and its page's scales
+struct TilePlace { long at; float ks, vs; };
+__device__ __forceinline__ TilePlace tile_place(const PagedAttnParams& p, int page, int tile, int h) {
+  if (page < 0) return {0, 1.f, 1.f};
+  const int per_page = p.t.page_shift - 6;
+  const long ph = (long)page * p.kv_heads + h;
+  return {(ph << per_page) + (tile & ((1 << per_page) - 1)), p.ks[ph], p.vs[ph]};
+}
+__device__ __forceinline__ bool sees_whole(const PagedAttnParams& p, long k0, long pos0, long pos1, long length) {
+  return k0 + 63 <= pos0 && k0 + 64 <= length && (p.window <= 0 || k0 > pos1 - p.window || k0 + 64 <= p.keep);
+}
+
+// Single tokens, and several: a workgroup takes 16 columns of one KV head and `split_tiles` tiles of 64 keys, its waves every fourth tile each; their results
+// meet in LDS. A wave has the next tile on its way to registers while it works on one: 16 KB (128 dimensions), 8 waves to a CU.
 template <typename T, int DC, int PIECES>
-__global__ void __launch_bounds__(256) paged_columns_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_columns_kernel(const PagedAttnParams p) {
   constexpr int D = DC * 64, W = 4;
   __shared__ float so[W][16][D + 4];
   __shared__ float sm[W][16], sl[W][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.z, h = blockIdx.y % p.kv_heads, ct = blockIdx.y / p.kv_heads;
-  const PagedSpan sp = paged_span(p.t, b);
-  const long n_cols = (long)sp.count * p.group;
-  if (16L * ct >= n_cols) return;
+  const PagedSpan sp = uniform(paged_span(p.t, b));
+  if (16 * ct >= sp.count * p.group) return;
+  const ColumnBlock cb = column_block(p, sp, ct, 16);
   const int g = lane >> 4;
-  const long col = 16L * ct + (lane & 15);
-  const bool there = col < n_cols;
-  const int token = (int)((there ? col : n_cols - 1) / p.group), head = h * p.group + (int)((there ? col : n_cols - 1) % p.group);
-  const long pos = there ? sp.start + token : -1;
-  const int token0 = (int)(16L * ct / p.group), token1 = (int)((16L * ct + 15 < n_cols ? 16L * ct + 15 : n_cols - 1) / p.group);
-  const TileRange range = tile_range(p, sp.start + token0, sp.start + token1, sp.length);
+  const int col = cb.first + (lane & 15);
+  const bool there = col < cb.end;
+  const int token = (unsigned)(there ? col : cb.end - 1) / (unsigned)p.group, head = h * p.group + (there ? col : cb.end - 1) - token * p.group;
+  const long pos[1] = {there ? sp.start + token : -1};
   const int begin = blockIdx.x * p.split_tiles;
-  const int n_tiles = range.count();
+  const int n_tiles = cb.range.count();
   if (begin >= n_tiles && begin > 0) return;
   const int end = begin + p.split_tiles < n_tiles ? begin + p.split_tiles : n_tiles;
 
-  QueryTile<DC, PIECES> q;
-  load_queries<T, DC, PIECES>(q, p.q + (long)(sp.row0 + token) * p.q_tok + (long)head * p.q_head, there, p.scale, g);
-  Columns<DC> c;
-  c.m = kNoMax;
-  c.l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4 * DC; ++i) c.o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Columns<DC> c[1];
+  c[0].clear();
   const int per_page = p.t.page_shift - 6;
+  auto page_of = [&](int i) { return i < end ? paged_page(p.t, b, cb.range.at(i) >> per_page) : -1; };
+  KvRegs<DC> t, next;
+  int page = page_of(begin + wave), page1 = page_of(begin + wave + W);
+  TilePlace at = tile_place(p, page, cb.range.at(begin + wave), h), at1;
+  if (page >= 0) t.load(p.kp + at.at * (64 * D), p.vp + at.at * (64 * D), lane);
+  QueryTile<DC, PIECES> q[1];
+  load_queries<T, DC, PIECES>(q[0], p.q + (long)(sp.row0 + token) * p.q_tok + (long)head * p.q_head, there, p.scale, g);
   for (int i = begin + wave; i < end; i += W) {
-    const int tile = range.at(i);
-    const int page = paged_page(p.t, b, tile >> per_page);
-    if (page < 0) continue;
-    const long ph = (long)page * p.kv_heads + h;
-    const long at = (ph << per_page) + (tile & ((1 << per_page) - 1));
-    KvTile<DC> t;
-    load_tile<DC>(t, p.kp + at * (64 * D), p.vp + at * (64 * D), lane);
-    const long k0 = 64L * tile;
-    const bool whole = k0 + 63 <= sp.start + token0 && k0 + 64 <= sp.length &&
-                       (p.window <= 0 || k0 > sp.start + token1 - p.window || k0 + 64 <= p.keep);
-    attend_tile<T, DC, PIECES>(c, q, t, p.ks[ph], p.vs[ph], whole, k0, pos, sp.length, p.window, p.keep, g);
+    const int page2 = page_of(i + 2 * W);
+    at1 = tile_place(p, page1, cb.range.at(i + W), h);
+    if (page1 >= 0) next.load(p.kp + at1.at * (64 * D), p.vp + at1.at * (64 * D), lane);
+    if (page >= 0) {
+      const long k0 = 64L * cb.range.at(i);
+      attend_tile<DC, PIECES, 1>(c, q, t, at.ks, at.vs, sees_whole(p, k0, cb.pos0, cb.pos1, sp.length), k0, pos, sp.length, p.window, p.keep, g);
+    }
+    t = next;
+    at = at1;
+    page = page1;
+    page1 = page2;
   }
-  const float l = rows_sum(c.l);
 #pragma unroll
-  for (int i = 0; i < 4 * DC; ++i) *(f32x4*)&so[wave][lane & 15][16 * i + 4 * g] = c.o[i];
-  if (g == 0) { sm[wave][lane & 15] = c.m; sl[wave][lane & 15] = l; }
+  for (int i = 0; i < 4 * DC; ++i) *(f32x4*)&so[wave][lane & 15][16 * i + 4 * g] = c[0].o[i];
+  if (g == 0) { sm[wave][lane & 15] = c[0].m; sl[wave][lane & 15] = c[0].l[0]; }
   __syncthreads();
   // 16 threads per column
   const int cc = threadIdx.x >> 4;
-  const long my = 16L * ct + cc;
-  if (my >= n_cols) return;
-  const int my_token = (int)(my / p.group), my_head = h * p.group + (int)(my % p.group);
+  const int my = cb.first + cc;
+  if (my >= cb.end) return;
+  const int my_token = (unsigned)my / (unsigned)p.group, my_head = h * p.group + my - my_token * p.group;
   float m = sm[0][cc];
 #pragma unroll
   for (int w = 1; w < W; ++w) m = fmaxf(m, sm[w][cc]);
@@ -322,6 +389,399 @@ __global__ void __launch_bounds__(256) paged_columns_kernel(const PagedAttnParam
   if (part && (threadIdx.x & 15) == 0) { part[D] = m; part[D + 1] = sum; }
 }
 
+// ---------------------------------------------------------------------------------------
+// prompts
+// ---------------------------------------------------------------------------------------
+// Here the vector ALU is what counts beside the matrix cores (an exponential per key and query), so probabilities go into the value products whole, in the queries'
+// type, and values are converted to it once for the workgroup: 16 conversions a thread and tile in place of 100 instructions of splitting and of operands put together.
+// A probability is taken relative to a power of two that moves only if a maximum passes it by kRoom: for fp16 so that the largest are 2^7 to 2^15, what is 2^-21 of
+// the largest still has all its bits and what is 2^-31 of it some; bf16 has the exponents for anything.
+template <typename T> struct PromptType;
+template <> struct PromptType<BF16> {
+  static constexpr float kBias = 0.f, kRoom = 60.f;
+  static constexpr uint32_t kOne = 0x3f80u;
+  static __device__ __forceinline__ uint32_t codes(uint32_t w, float s, bool high) {
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true)) : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
+  }
+};
+template <> struct PromptType<F16> {
+  static constexpr float kBias = 7.f, kRoom = 8.f;
+  static constexpr uint32_t kOne = 0x3c00u;
+  static __device__ __forceinline__ uint32_t codes(uint32_t w, float s, bool high) {
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true)) : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false));
+  }
+};
+
+// x *= f where it stands: a multiplication behind a branch would have the compiler copy every result on the other way round it. What it does not see into it does not
+// space from others either, so between_matrix() stands in front of such products, behind the instructions that make f, and behind them: 24 waits cover a matrix
+// instruction that writes x (16 passes: 19) and the exponential that gives f (1).
+__device__ __forceinline__ void between_matrix() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void times_here(f32x4& x, float f) {
+  float a = x[0], b = x[1], c = x[2], d = x[3];
+  asm volatile("v_mul_f32 %0, %4, %0\n\tv_mul_f32 %1, %4, %1\n\tv_mul_f32 %2, %4, %2\n\tv_mul_f32 %3, %4, %3" : "+v"(a), "+v"(b), "+v"(c), "+v"(d) : "v"(f));
+  x = f32x4{a, b, c, d};
+}
+
+template <int DC>
+struct PromptColumns {
+  f32x4 o[4 * DC];
+  f32x4 l;      // the sum of the probabilities, as they went into the products: four times the same
+  float m, to;  // what probabilities are relative to: 2^m; kBias - m
+};
+
+// a tile in LDS as a wave's lanes have its operands: keys as codes (chunk i: 16 keys and 64 dimensions), values in the queries' type (16 dimensions, 32 keys)
+struct PromptTile {
+  const u32x4* kp; const u32x4* vp;
+  __device__ __forceinline__ u32x4 k(int i) const { return kp[i * 64]; }
+  __device__ __forceinline__ u32x4 v(int i, int half) const { return vp[(2 * i + half) * 64]; }
+};
+
+// scores of a tile
+template <int DC, int PIECES, int NT>
+__device__ __forceinline__ void prompt_scores(f32x4 (&s)[NT][4], const QueryTile<DC, PIECES> (&q)[NT], const PromptTile& t) {
+  constexpr int M = (DC + 1) / 2;
+  const u32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {  // (two chunks' products between one product and the next on its result)
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      i32x8 kk[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) kk[k] = pair8(t.k(8 * m + i + k), 2 * m + 1 < DC ? t.k(2 * m + 1 < DC ? 8 * m + 4 + i + k : 0) : zero);
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s[n][i + k] = mfma_e4m3(kk[k], q[n].piece[j][m], m || j ? s[n][i + k] : f32x4{0.f, 0.f, 0.f, 0.f}, 127, 127 - 5 * j);
+    }
+  }
+}
+
+// keys 16 i + 4 g + r of a tile that a query sees: bit 4 i + r
+__device__ __forceinline__ uint32_t seen_bits(long first_key, long pos, long length, int window, int keep, int g) {
+  const unsigned long long m = seen_keys(first_key, pos, length, window, keep, g);
+  return (uint32_t)(m & 0xf) | (uint32_t)(m >> 16 & 0xf) << 4 | (uint32_t)(m >> 32 & 0xf) << 8 | (uint32_t)(m >> 48 & 0xf) << 12;
+}
+
+// The reference of the probabilities moves where the tile's largest score (of this lane's keys) passes it by kRoom.
+template <typename T, int DC, int NT>
+__device__ __forceinline__ void prompt_move(PromptColumns<DC> (&c)[NT], const float (&most)[NT]) {
+  typedef PromptType<T> PT;
+  bool moves = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) moves |= most[n] > c[n].m + PT::kRoom;
+  if (__any(moves)) {
+    float f[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {  // (a column's four lanes move together)
+      const float mt = fmaxf(ceilf(fminf(rows_max(most[n]), 1e30f)), kNoMax), to = mt > c[n].m + PT::kRoom ? mt : c[n].m;
+      f[n] = __builtin_amdgcn_exp2f(c[n].m - to);
+      c[n].m = to;
+      c[n].to = fabsf(to) < 1e8f ? PT::kBias - to : -to;  // (beyond, the sum would be rounded)
+    }
+    between_matrix();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      times_here(c[n].l, f[n]);
+#pragma unroll
+      for (int i = 0; i < 4 * DC; ++i) times_here(c[n].o[i], f[n]);
+    }
+    between_matrix();
+  }
+}
+
+template <int NT>
+__device__ __forceinline__ void prompt_most(float (&most)[NT], const f32x4 (&s)[NT][4]) {
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    most[n] = s[n][0][0];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) most[n] = fmaxf(most[n], s[n][i][r]);
+  }
+}
+
+// probabilities of a tile: unit = what its scores are multiplied by
+template <typename T, int DC, int NT>
+__device__ __forceinline__ void prompt_exp(u32x4 (&pp)[NT][2], const f32x4 (&s)[NT][4], const PromptColumns<DC> (&c)[NT], const float (&unit)[NT]) {
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float e[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[n][i][r], unit[n], c[n].to));
+      pp[n][i >> 1][2 * (i & 1)] = T::pack2(e[0], e[1]);
+      pp[n][i >> 1][2 * (i & 1) + 1] = T::pack2(e[2], e[3]);
+    }
+}
+
+template <typename T, int DC, int NT>
+__device__ __forceinline__ void prompt_values(PromptColumns<DC> (&c)[NT], const u32x4 (&pp)[NT][2], const PromptTile& t) {
+  constexpr uint32_t kOnes = PromptType<T>::kOne * 0x10001u;
+  const u32x4 ones = {kOnes, kOnes, kOnes, kOnes};
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) c[n].l = mfma16x16x32<T>(ones, pp[n][half], c[n].l);
+#pragma unroll
+  for (int i = 0; i < 4 * DC; ++i)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const u32x4 v = t.v(i, half);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) c[n].o[i] = mfma16x16x32<T>(v, pp[n][half], c[n].o[i]);
+    }
+}
+
+// Where part of a tile is hidden its NaN codes have gone into the products as zeros, since 0 * NaN is NaN: here the columns that see one get a NaN. v: the tile's values.
+template <int DC, int NT>
+__device__ __forceinline__ void prompt_nans(PromptColumns<DC> (&c)[NT], const uint8_t* v, const uint32_t (&seen)[NT]) {
+  const u32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 4 * DC; ++i) {
+    __builtin_amdgcn_sched_barrier(0);  // (one chunk at a time: kept apart, these rare steps cost the others no registers)
+    u32x4 x = ld16(v + i * 1024);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = nan_bytes(x[j]) & 0x38383838u;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      u32x4 mine;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w |= seen[n] >> (4 * k + r) & 1u ? 0x38u << (8 * r) : 0u;
+        mine[k] = w;
+      }
+      const f32x4 sees = mfma_e4m3(pair8(x, zero), pair8(mine, zero), f32x4{0.f, 0.f, 0.f, 0.f}, 127, 127);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) c[n].o[i][r] = sees[r] > 0.f ? __builtin_nanf("") : c[n].o[i][r];
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// A workgroup of W waves takes W NT times 16 columns of one KV head (NT times 16 a wave) and `split_tiles` tiles, which its waves share through LDS: two tiles' room, the
+// next one's keys on their way to LDS and its values to registers while the waves work on one, one barrier a tile.
+template <typename T, int DC, int PIECES, int NT, int W>
+__global__ void __launch_bounds__(64 * W, W / 4 * (DC == 4 ? 1 : 2)) paged_tiles_kernel(const PagedAttnParams p) {
+  constexpr int D = DC * 64, kCols = 16 * W * NT, kMine = (4 * DC + W - 1) / W;  // chunks of a tile that a wave fetches
+  typedef PromptType<T> PT;
+  __shared__ u32x4 keys[2][64 * D / 16], values[2][64 * D / 8];
+  __shared__ int nan_tile[2];  // number of the tile + 1 where its values hold a NaN (looked for, and taken out, where not every column sees all of it)
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Neighbouring blocks go to different XCDs: those of one request and KV head, which read the same keys, lie a multiple of n_requests * kv_heads apart. The
+  // last columns see most: they come first.
+  const unsigned units = p.t.n_requests * p.kv_heads;
+  const int b = blockIdx.x % units / p.kv_heads, h = blockIdx.x % units % p.kv_heads, ct = p.col_tiles - 1 - blockIdx.x / units;
+  const PagedSpan sp = uniform(paged_span(p.t, b));
+  if (kCols * ct >= sp.count * p.group) return;
+  const ColumnBlock cb = column_block(p, sp, ct, kCols);
+  const int n_tiles = cb.range.count();
+  const int begin = blockIdx.y * p.split_tiles;
+  if (begin >= n_tiles && begin > 0) return;
+  const int end = begin + p.split_tiles < n_tiles ? begin + p.split_tiles : n_tiles;
+  const int g = lane >> 4;
+  if (threadIdx.x < 2) nan_tile[threadIdx.x] = 0;
+  QueryTile<DC, PIECES> q[NT];
+  PromptColumns<DC> c[NT];
+  int token[NT];  // of the request's new ones, the lane's columns'; -1: no column
+  const int wave_col = cb.first + wave * (16 * NT);
+  const bool mine = wave_col < cb.end;
+  const int wave_end = wave_col + 16 * NT < cb.end ? wave_col + 16 * NT : cb.end;
+  const long my_pos1 = sp.start + (unsigned)(mine ? wave_end - 1 : cb.end - 1) / (unsigned)p.group;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int col = wave_col + 16 * n + (lane & 15);
+    const bool there = col < cb.end;
+    const unsigned at = there ? col : cb.end - 1, tok = at / (unsigned)p.group, head = at - tok * p.group;
+    token[n] = there ? (int)tok : -1;
+    load_queries<T, DC, PIECES>(q[n], p.q + (long)(sp.row0 + (int)tok) * p.q_tok + (long)(h * p.group + (int)head) * p.q_head, there, p.scale, g);
+#pragma unroll
+    for (int i = 0; i < 4 * DC; ++i) c[n].o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    c[n].l = f32x4{0.f, 0.f, 0.f, 0.f};
+    c[n].m = kNoMax;
+    c[n].to = -kNoMax;
+  }
+  const int per_page = p.t.page_shift - 6;
+  const int lane_at = (lane & 15) * 64 + (lane >> 4) * 16;
+  auto page_of = [&](int i) { return i < end ? __builtin_amdgcn_readfirstlane(paged_page(p.t, b, cb.range.at(i) >> per_page)) : -1; };
+  auto fetch_keys = [&](const TilePlace& at, int slot) {
+    if (4 * DC < W && wave >= 4 * DC) return;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      load_lds16((const uint16_t*)(p.kp + at.at * (64 * D) + (wave * kMine + i) * 1024 + lane_at), (uint16_t*)&keys[slot][(wave * kMine + i) * 64]);
+  };
+  u32x4 raw[kMine];
+  auto fetch_values = [&](const TilePlace& at) {
+    if (4 * DC < W && wave >= 4 * DC) return;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) raw[i] = ld16(p.vp + at.at * (64 * D) + (wave * kMine + i) * 1024 + lane_at);
+  };
+  // fp16 holds a page's values times 2^(7 - loudest) of the loudest page so far: all codes exactly, unless a page is 2^22 times quieter than another
+  int loudest = -126;
+  auto put_values = [&](const TilePlace& at, int slot, int tile_no) {
+    if (!sees_whole(p, 64L * cb.range.at(tile_no), cb.pos0, cb.pos1, sp.length)) {
+      uint32_t found = 0;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t n = nan_bytes(raw[i][j]);
+          found |= n;
+          raw[i][j] &= ~n;
+        }
+      if (__any(found != 0) && lane == 0) nan_tile[slot] = tile_no + 1;
+    }
+    float s = at.vs;
+    if constexpr (T::kDtype == MUI_DTYPE_F16) {
+      const int e = scale_exponent(at.vs);
+      if (e > loudest) {
+        const float f = exp2i(loudest - e < -126 ? -126 : loudest - e);
+        between_matrix();
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4 * DC; ++i) times_here(c[n].o[i], f);
+        between_matrix();
+        loudest = e;
+      }
+      s = exp2i(e - loudest + 7 < -126 ? -126 : e - loudest + 7);
+    }
+    if (4 * DC < W && wave >= 4 * DC) return;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t a = raw[i][2 * half], d = raw[i][2 * half + 1];
+        values[slot][((wave * kMine + i) * 2 + half) * 64 + lane] = u32x4{PT::codes(a, s, false), PT::codes(a, s, true), PT::codes(d, s, false), PT::codes(d, s, true)};
+      }
+  };
+  // Tile i's probabilities and value products go with tile i + 1's scores: while the vector ALU takes exponentials the matrix cores have products that wait for nothing.
+  // A step begins with tile i's scores in registers, its values in LDS or about to be, tile i + 1's keys on their way to LDS.
+  int page = page_of(begin), page1 = page_of(begin + 1), page2 = page_of(begin + 2);
+  TilePlace at = tile_place(p, page, cb.range.at(begin), h), at1 = tile_place(p, page1, cb.range.at(begin + 1), h);
+  f32x4 s[NT][4];
+  float most[NT], unit[NT];
+  __syncthreads();  // (nan_tile)
+  if (page >= 0) {
+    fetch_keys(at, 0);
+    fetch_values(at);
+    put_values(at, 0, begin);
+  }
+  wait_loads<0>();
+  __syncthreads();
+  if (page1 >= 0) fetch_keys(at1, 1);
+  // scores that may be hidden: tile number, its place in LDS, whether it has a page
+  auto masked_scores = [&](int tile_no, int slot, bool there) {
+    const long k0 = 64L * cb.range.at(tile_no);
+    if (there && mine && k0 <= my_pos1) prompt_scores<DC, PIECES, NT>(s, q, PromptTile{&keys[slot][lane], nullptr});
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const uint32_t seen = there && mine ? seen_bits(k0, token[n] < 0 ? -1 : sp.start + token[n], sp.length, p.window, p.keep, g) : 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[n][i][r] = seen >> (4 * i + r) & 1u ? s[n][i][r] : -INFINITY;
+    }
+  };
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (begin < end) {
+    masked_scores(begin, 0, page >= 0);
+    prompt_most<NT>(most, s);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      unit[n] = q[n].unit * at.ks;
+      most[n] *= unit[n];
+    }
+    prompt_move<T, DC, NT>(c, most);
+  }
+  int i = begin;
+  auto step = [&](auto whole) {
+    constexpr bool kWhole = decltype(whole)::value;  // all columns see all of tiles i and i + 1
+    const int slot = (i - begin) & 1;
+    wait_loads<0>();
+    __syncthreads();  // tile i's values and tile i + 1's keys are there, for all; the other rooms' readers are done
+    const int page3 = page_of(i + 3);
+    const TilePlace at2 = tile_place(p, page2, cb.range.at(i + 2), h);
+    if (page2 >= 0) fetch_keys(at2, slot);
+    if (page1 >= 0) fetch_values(at1);
+    u32x4 pp[NT][2];
+    const PromptTile here = {nullptr, &values[slot][lane]}, ahead = {&keys[slot ^ 1][lane], nullptr};
+    prompt_exp<T, DC, NT>(pp, s, c, unit);
+    if constexpr (kWhole) {
+      prompt_scores<DC, PIECES, NT>(s, q, ahead);
+      prompt_values<T, DC, NT>(c, pp, here);
+    } else {
+      if (i + 1 < end) masked_scores(i + 1, slot ^ 1, page1 >= 0);
+      const long k0 = 64L * cb.range.at(i);
+      if (page >= 0 && mine && k0 <= my_pos1) {
+        prompt_values<T, DC, NT>(c, pp, here);
+        if (nan_tile[slot] == i + 1) {
+          uint32_t seen[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) seen[n] = seen_bits(k0, token[n] < 0 ? -1 : sp.start + token[n], sp.length, p.window, p.keep, g);
+          prompt_nans<DC, NT>(c, p.vp + tile_place(p, page, cb.range.at(i), h).at * (64 * D) + lane_at, seen);
+        }
+      }
+    }
+    prompt_most<NT>(most, s);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      unit[n] = q[n].unit * at1.ks;
+      most[n] *= unit[n];
+    }
+    if (page1 >= 0) put_values(at1, slot ^ 1, i + 1);
+    if (kWhole || i + 1 < end) prompt_move<T, DC, NT>(c, most);
+    at1 = at2;
+    page = page1;
+    page1 = page2;
+    page2 = page3;
+    ++i;
+  };
+  // (a loop for tiles that all columns see and one for others: with both in one the compiler copied the results between their registers at every tile)
+  auto whole_now = [&]() {
+    return i + 1 < end && page >= 0 && page1 >= 0 && sees_whole(p, 64L * cb.range.at(i), cb.pos0, cb.pos1, sp.length) &&
+           sees_whole(p, 64L * cb.range.at(i + 1), cb.pos0, cb.pos1, sp.length);
+  };
+  while (i < end) {
+    while (whole_now()) step(std::true_type());
+    while (i < end && !whole_now()) step(std::false_type());
+  }
+  const float loud = T::kDtype == MUI_DTYPE_F16 ? exp2i(loudest - 7 < -126 ? -126 : loudest - 7) : 1.f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int col = wave_col + 16 * n + (lane & 15);
+    if (col >= cb.end) continue;
+    const unsigned token = (unsigned)col / (unsigned)p.group;
+    const long row = (long)(sp.row0 + (int)token) * p.heads + h * p.group + (col - (int)token * p.group);
+    const float sum = c[n].l[0];
+    if (p.part) {
+      float* part = p.part + ((long)blockIdx.y * p.t.n_rows * p.heads + row) * (D + 4);
+#pragma unroll
+      for (int i = 0; i < 4 * DC; ++i) *(f32x4*)(part + 16 * i + 4 * g) = c[n].o[i] * loud;
+      if (g == 0) { part[D] = -c[n].to; part[D + 1] = sum; }
+    } else {
+      const float inv = sum > 0.f || sum != sum ? loud / sum : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4 * DC; ++i) {
+        const f32x4 o = c[n].o[i] * inv;
+        *(u32x2*)(p.out + row * D + 16 * i + 4 * g) = u32x2{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])};
+      }
+    }
+  }
+}
+
 // The splits of a row and head together: a wave each.
 template <typename T, int DC>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p) {
@@ -342,12 +802,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   }
   const PagedSpan sp = paged_span(p.t, b);
   if (row < sp.row0 || row >= sp.row0 + sp.count) return;
-  // the tiles of the row's column tile, as the kernel above has them
-  const int token = row - sp.row0;
-  const long ct = ((long)token * p.group + head % p.group) / 16;
-  const long n_cols = (long)sp.count * p.group;
-  const int token0 = (int)(16L * ct / p.group), token1 = (int)((16L * ct + 15 < n_cols ? 16L * ct + 15 : n_cols - 1) / p.group);
-  const int n_tiles = tile_range(p, sp.start + token0, sp.start + token1, sp.length).count();
+  const int col = (row - sp.row0) * p.group + head % p.group;
+  const int n_tiles = column_block(p, sp, col / p.block_cols, p.block_cols).range.count();
   int splits = n_tiles > 0 ? (n_tiles + p.split_tiles - 1) / p.split_tiles : 1;
   splits = splits < p.splits ? splits : p.splits;
   const float* part = p.part + item * (D + 4);
@@ -366,11 +822,13 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   for (int j = 0; j < DC; ++j) p.out[item * D + 64 * j + lane] = T::pack(o[j] * inv);
 }
 
-struct PagedPlan { int col_tiles, split_tiles, splits; };
-static PagedPlan paged_plan(int n_requests, int max_tokens, int max_length, int window, int keep, int n_q_heads, int n_kv_heads) {
+struct PagedPlan { int block_cols, col_tiles, split_tiles, splits; };
+static PagedPlan paged_plan(int n_requests, int max_tokens, int max_length, int window, int keep, int n_q_heads, int n_kv_heads, int head_dim) {
   PagedPlan r;
   const long group = n_q_heads / n_kv_heads;
-  r.col_tiles = (int)((max_tokens * group + 15) / 16);
+  const bool prompt = max_tokens * group > 64;
+  r.block_cols = prompt ? (head_dim == 256 ? 64 : 128) : 16;  // (256 dimensions: results of 32 columns a wave do not fit its registers)
+  r.col_tiles = (int)((max_tokens * group + r.block_cols - 1) / r.block_cols);
   long tiles = ((long)max_length + 63) / 64;
   if (window > 0) {
     const long seen = ((long)window + max_tokens + 62) / 64 + 1 + ((long)keep + 63) / 64;
@@ -378,7 +836,7 @@ static PagedPlan paged_plan(int n_requests, int max_tokens, int max_length, int 
   }
   if (tiles < 1) tiles = 1;
   const long work = (long)n_requests * n_kv_heads * r.col_tiles;
-  long splits = (1024 + work - 1) / work;
+  long splits = prompt ? (512 + work - 1) / work : (1024 + work - 1) / work;
   if (splits > (tiles + 7) / 8) splits = (tiles + 7) / 8;
   if (splits < 1) splits = 1;
   r.split_tiles = (int)((tiles + splits - 1) / splits);
@@ -398,7 +856,7 @@ static bool paged_attention_sizes(int n_rows, int n_requests, int max_tokens, in
 extern "C" size_t mui_paged_attention_scratch_bytes(int n_rows, int n_requests, int max_tokens, int max_length, int window, int keep_first, int n_q_heads,
                                                     int n_kv_heads, int head_dim) {
   if (!paged_attention_sizes(n_rows, n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads, head_dim)) return 0;
-  const PagedPlan plan = paged_plan(n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads);
+  const PagedPlan plan = paged_plan(n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads, head_dim);
   return plan.splits > 1 ? (size_t)plan.splits * n_rows * n_q_heads * (head_dim + 4) * 4 : 0;
 }
 
@@ -417,9 +875,12 @@ extern "C" int mui_paged_attention(mui_stream_t stream, int dtype, const void* q
   if ((q_token_stride | q_head_stride) & 7) return MUI_ERR_ALIGNMENT;
   const long cap = (long)table_pages * page_tokens;
   if (max_length > cap) max_length = (int)cap;
-  const PagedPlan plan = paged_plan(n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads);
+  const PagedPlan plan = paged_plan(n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads, head_dim);
   if (plan.splits > 1 && (!scratch || scratch_bytes < (size_t)plan.splits * n_rows * n_q_heads * (head_dim + 4) * 4)) return MUI_ERR_INVALID_ARG;
-  if ((long)plan.col_tiles * n_kv_heads > 65535 || n_requests > 65535) return MUI_ERR_UNSUPPORTED;
+  if ((long)n_rows * n_q_heads > 0x7fffffffL - 256) return MUI_ERR_UNSUPPORTED;
+  const bool prompt = plan.block_cols > 16;
+  const long blocks = (long)plan.col_tiles * n_kv_heads * n_requests;
+  if (blocks > 0x7fffffffL || plan.splits > 65535 || n_requests > 65535 || (!prompt && (long)plan.col_tiles * n_kv_heads > 65535)) return MUI_ERR_UNSUPPORTED;
   PagedAttnParams p = {};
   p.q = (const uint16_t*)q; p.q_tok = q_token_stride; p.q_head = q_head_stride;
   p.kp = (const uint8_t*)k_pages; p.vp = (const uint8_t*)v_pages; p.ks = k_scale; p.vs = v_scale;
@@ -427,7 +888,7 @@ extern "C" int mui_paged_attention(mui_stream_t stream, int dtype, const void* q
   p.scale = scale * 1.4426950408889634f;
   p.window = window; p.keep = window > 0 ? keep_first : 0;
   p.heads = n_q_heads; p.kv_heads = n_kv_heads; p.group = n_q_heads / n_kv_heads;
-  p.col_tiles = plan.col_tiles; p.split_tiles = plan.split_tiles; p.splits = plan.splits;
+  p.block_cols = plan.block_cols; p.col_tiles = plan.col_tiles; p.split_tiles = plan.split_tiles; p.splits = plan.splits;
   p.part = plan.splits > 1 ? (float*)scratch : nullptr;
   p.out = (uint16_t*)out;
   hipStream_t s = (hipStream_t)stream;
@@ -435,7 +896,10 @@ extern "C" int mui_paged_attention(mui_stream_t stream, int dtype, const void* q
   const dim3 join((unsigned)(((long)n_rows * n_q_heads + 3) / 4));
 #define MUI_PAGED_GO(TT, DC, PIECES)                                                                     \
   do {                                                                                                   \
-    hipLaunchKernelGGL((paged_columns_kernel<TT, DC, PIECES>), grid, dim3(256), 0, s, p);                \
+    if (prompt)                                                                                          \
+      hipLaunchKernelGGL((paged_tiles_kernel<TT, DC, PIECES, DC == 4 ? 1 : 2, 4>), dim3((unsigned)blocks, plan.splits), dim3(256), 0, s, p); \
+    else                                                                                                 \
+      hipLaunchKernelGGL((paged_columns_kernel<TT, DC, PIECES>), grid, dim3(256), 0, s, p);              \
     if (plan.splits > 1) hipLaunchKernelGGL((paged_join_kernel<TT, DC>), join, dim3(256), 0, s, p);      \
   } while (0)
 #define MUI_PAGED_TYPES(DC) \
