@@ -25,11 +25,37 @@ struct PagedAttnParams {
   int col_tiles;        // such blocks of a request at most
   int split_tiles;      // tiles of 64 keys per workgroup
   int splits;           // at most
-  float* part;          // [splits][n_rows * heads][dim + 2], or null: one split
+  float* part;          // partial results, or null: none. Single tokens: [workgroups][2][16][dim + 4], prompts [splits][n_rows * heads][dim + 4]; dim values, maximum, sum
+  int* before;          // [n_requests + 1], single tokens: see paged_columns_kernel
   uint16_t* out;
 };
 
 constexpr float kNoMax = -1e30f;
+constexpr int kDealtRequests = 1024;  // requests whose tiles are dealt out (more give a workgroup each anyway)
+
+// tiles of a workgroup's share, at least one a wave
+__device__ __forceinline__ int share_of(int total, int workgroups, int waves) {
+  const int s = (total + workgroups - 1) / workgroups;
+  return s > waves ? s : waves;
+}
+
+// the last request whose rows begin at or before `row`
+__device__ __forceinline__ int request_of(const PagedTable& t, int row) {
+  if (!t.offsets) return row;
+  int lo = 0, hi = t.n_requests;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.offsets[mid] <= row) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// (what a request's numbers say is the same for a workgroup, which the compiler does not see where they come from memory: in scalar registers it costs the results no room)
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long uniform(long x) {
+  return (long)((unsigned long long)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)(x & 0xffffffffL)));
+}
+__device__ __forceinline__ PagedSpan uniform(PagedSpan s) { return {uniform(s.row0), uniform(s.count), uniform(s.start), uniform(s.length)}; }
 
 // The tiles of 64 keys that queries at positions first .. last see: `kept` from the beginning, then those from `from` to `end`.
 struct TileRange { int kept, from, end; __device__ int count() const { return kept + (end > from ? end - from : 0); }
@@ -63,16 +89,28 @@ struct QueryTile {
   i32x8 piece[PIECES][M];
   float unit;  // what the products are multiplied by, the score scale included
 };
+template <int DC>
+struct QueryRow { u32x4 v[DC][2]; };
+template <int DC>
+__device__ __forceinline__ QueryRow<DC> request_queries(const uint16_t* row, int g) {
+  QueryRow<DC> r;
+#pragma unroll
+  for (int c = 0; c < DC; ++c) {
+    r.v[c][0] = ld16(row + c * 64 + g * 16);
+    r.v[c][1] = ld16(row + c * 64 + g * 16 + 8);
+  }
+  return r;
+}
 template <typename T, int DC, int PIECES>
-__device__ __forceinline__ void load_queries(QueryTile<DC, PIECES>& t, const uint16_t* row, bool there, float score_scale, int g) {
+__device__ __forceinline__ void take_queries(QueryTile<DC, PIECES>& t, const QueryRow<DC>& row, bool there, float score_scale, int g) {
   float x[DC][16];
   float most = 0.f;
 #pragma unroll
   for (int c = 0; c < DC; ++c) {
     const u32x4 zero = {0, 0, 0, 0};
     float a[8], b[8];
-    unpack8<T>(there ? ld16(row + c * 64 + g * 16) : zero, a);
-    unpack8<T>(there ? ld16(row + c * 64 + g * 16 + 8) : zero, b);
+    unpack8<T>(there ? row.v[c][0] : zero, a);
+    unpack8<T>(there ? row.v[c][1] : zero, b);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       x[c][i] = a[i];
@@ -290,13 +328,6 @@ __device__ __forceinline__ ColumnBlock column_block(const PagedAttnParams& p, co
   return b;
 }
 
-// (what a request's numbers say is the same for a workgroup, which the compiler does not see where they come from memory: in scalar registers it costs the results no room)
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ long uniform(long x) {
-  return (long)((unsigned long long)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)(x & 0xffffffffL)));
-}
-__device__ __forceinline__ PagedSpan uniform(PagedSpan s) { return {uniform(s.row0), uniform(s.count), uniform(s.start), uniform(s.length)}; }
-
 // where a tile lies, and its page's scales
 struct TilePlace { long at; float ks, vs; };
 __device__ __forceinline__ TilePlace tile_place(const PagedAttnParams& p, int page, int tile, int h) {
@@ -309,84 +340,209 @@ __device__ __forceinline__ bool sees_whole(const PagedAttnParams& p, long k0, lo
   return k0 + 63 <= pos0 && k0 + 64 <= length && (p.window <= 0 || k0 > pos1 - p.window || k0 + 64 <= p.keep);
 }
 
-// Single tokens, and several: a workgroup takes 16 columns of one KV head and `split_tiles` tiles of 64 keys, its waves every fourth tile each; their results
-// meet in LDS. A wave has the next tile on its way to registers while it works on one: 16 KB (128 dimensions), 8 waves to a CU.
-template <typename T, int DC, int PIECES>
-__global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_columns_kernel(const PagedAttnParams p) {
-  constexpr int D = DC * 64, W = 4;
+// A request's tiles of 64 keys that any of its new tokens sees (at least one, so that a token without keys gets its zeros) and its blocks of 16 columns; not
+// more than the host has been told, so that the sums over all requests fit.
+struct RequestWork { int tiles, blocks; };
+__device__ __forceinline__ RequestWork request_work(const PagedAttnParams& p, const PagedSpan& sp) {
+  RequestWork w = {0, (sp.count * p.group + 15) / 16};
+  if (sp.count > 0) w.tiles = tile_range(p, sp.start, sp.start + sp.count - 1, sp.length).count();
+  w.tiles = w.tiles < 1 ? 1 : w.tiles < p.split_tiles ? w.tiles : p.split_tiles;
+  w.blocks = w.blocks < p.col_tiles ? w.blocks : p.col_tiles;
+  return w;
+}
+
+// Single tokens, and several. A unit is 16 columns of one KV head and request. All tiles of all units, one after another, are dealt out to the workgroups in
+// equal shares, whatever the requests' lengths: the units that a share cuts are joined by a second launch. (Short caches: a workgroup per unit, nothing to join.) The waves of
+// a workgroup take every W-th tile each and meet in LDS. Two waves on a SIMD keep the memory busy, 16 KB on the way for each (128 dimensions): with the next tile requested
+// while one is worked on as well their registers do not suffice (64 requests of 4096 to 16384 tokens 204 instead of 190 us).
+template <typename T, int DC, int PIECES, int W>
+__global__ void __launch_bounds__(64 * W, DC == 4 ? W / 4 : 2) paged_columns_kernel(const PagedAttnParams p) {
+  constexpr int D = DC * 64, kThreads = 64 * W;
   __shared__ float so[W][16][D + 4];
   __shared__ float sm[W][16], sl[W][16];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.z, h = blockIdx.y % p.kv_heads, ct = blockIdx.y / p.kv_heads;
-  const PagedSpan sp = uniform(paged_span(p.t, b));
-  if (16 * ct >= sp.count * p.group) return;
-  const ColumnBlock cb = column_block(p, sp, ct, 16);
-  const int g = lane >> 4;
-  const int col = cb.first + (lane & 15);
-  const bool there = col < cb.end;
-  const int token = (unsigned)(there ? col : cb.end - 1) / (unsigned)p.group, head = h * p.group + (there ? col : cb.end - 1) - token * p.group;
-  const long pos[1] = {there ? sp.start + token : -1};
-  const int begin = blockIdx.x * p.split_tiles;
-  const int n_tiles = cb.range.count();
-  if (begin >= n_tiles && begin > 0) return;
-  const int end = begin + p.split_tiles < n_tiles ? begin + p.split_tiles : n_tiles;
-
-  Columns<DC> c[1];
-  c[0].clear();
+  __shared__ int before[kDealtRequests + 1];  // tiles of the units of the requests in front of each
+  __shared__ int wave_sum[W];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+  int b, unit = 0, tile0 = 0, share_begin = 0, share_end = 0, share = 0;
+  if (p.part) {
+    int mine[kDealtRequests / kThreads], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kDealtRequests / kThreads; ++k) {
+      const int r = threadIdx.x * (kDealtRequests / kThreads) + k;
+      if (r < p.t.n_requests) {
+        const RequestWork w = request_work(p, paged_span(p.t, r));
+        sum += w.tiles * w.blocks * p.kv_heads;
+      }
+      mine[k] = sum;
+    }
+    int to = sum;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(to, off);
+      if (lane >= off) to += o;
+    }
+    if (lane == 63) wave_sum[wave] = to;
+    __syncthreads();
+    int base = to - sum;
+    for (int w = 0; w < wave; ++w) base += wave_sum[w];
+#pragma unroll
+    for (int k = 0; k < kDealtRequests / kThreads; ++k) before[threadIdx.x * (kDealtRequests / kThreads) + k + 1] = base + mine[k];
+    if (threadIdx.x == 0) before[0] = 0;
+    __syncthreads();
+    const int total = uniform(before[p.t.n_requests]);
+    share = share_of(total, gridDim.x, W);
+    if (blockIdx.x == 0)  // for the joining launch
+      for (int i = threadIdx.x; i <= p.t.n_requests; i += kThreads) p.before[i] = before[i];
+    share_begin = (int)blockIdx.x * share;  // (share * workgroups < total + workgroups, which the host has checked)
+    share_end = total - share_begin < share ? total : share_begin + share;
+    if (share_begin >= total) return;
+    int lo = 0, hi = p.t.n_requests;  // the last request that begins at or before the share
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before[mid] <= share_begin) lo = mid; else hi = mid;
+    }
+    b = uniform(lo);
+  } else {
+    unit = blockIdx.x % (p.kv_heads * p.col_tiles);
+    b = blockIdx.x / (p.kv_heads * p.col_tiles);
+  }
+  PagedSpan sp = uniform(paged_span(p.t, b));
+  RequestWork work = request_work(p, sp);
+  int done = share_begin;
+  if (p.part) {
+    unit = (done - uniform(before[b])) / work.tiles;
+    tile0 = done - uniform(before[b]) - unit * work.tiles;
+  } else if (unit >= work.blocks * p.kv_heads) {
+    return;
+  }
   const int per_page = p.t.page_shift - 6;
-  auto page_of = [&](int i) { return i < end ? paged_page(p.t, b, cb.range.at(i) >> per_page) : -1; };
-  KvRegs<DC> t, next;
-  int page = page_of(begin + wave), page1 = page_of(begin + wave + W);
-  TilePlace at = tile_place(p, page, cb.range.at(begin + wave), h), at1;
-  if (page >= 0) t.load(p.kp + at.at * (64 * D), p.vp + at.at * (64 * D), lane);
-  QueryTile<DC, PIECES> q[1];
-  load_queries<T, DC, PIECES>(q[0], p.q + (long)(sp.row0 + token) * p.q_tok + (long)head * p.q_head, there, p.scale, g);
-  for (int i = begin + wave; i < end; i += W) {
-    const int page2 = page_of(i + 2 * W);
-    at1 = tile_place(p, page1, cb.range.at(i + W), h);
-    if (page1 >= 0) next.load(p.kp + at1.at * (64 * D), p.vp + at1.at * (64 * D), lane);
-    if (page >= 0) {
-      const long k0 = 64L * cb.range.at(i);
-      attend_tile<DC, PIECES, 1>(c, q, t, at.ks, at.vs, sees_whole(p, k0, cb.pos0, cb.pos1, sp.length), k0, pos, sp.length, p.window, p.keep, g);
+  while (true) {
+    // the unit's tiles tile0 .. tile0 + n - 1
+    const int n = p.part && share_end - done < work.tiles - tile0 ? share_end - done : work.tiles - tile0;
+    const bool all = n == work.tiles;
+    const int h = unit % p.kv_heads;
+    const ColumnBlock cb = column_block(p, sp, unit / p.kv_heads, 16);
+    const TileRange range = tile_range(p, sp.start, sp.start + sp.count - 1, sp.length);  // of the request
+    const int end = tile0 + n < range.count() ? tile0 + n : range.count();
+    const int col = cb.first + (lane & 15);
+    const bool there = col < cb.end;
+    const int token = (unsigned)(there ? col : cb.end - 1) / (unsigned)p.group, head = h * p.group + (there ? col : cb.end - 1) - token * p.group;
+    const long pos[1] = {there ? sp.start + token : -1};
+    const QueryRow<DC> query = request_queries<DC>(p.q + (long)(sp.row0 + token) * p.q_tok + (long)head * p.q_head, g);
+    Columns<DC> c[1];
+    c[0].clear();
+    auto page_of = [&](int i) { return i < end ? paged_page(p.t, b, range.at(i) >> per_page) : -1; };
+    KvRegs<DC> t;
+    int page = page_of(tile0 + wave);
+    TilePlace at = tile_place(p, page, range.at(tile0 + wave), h);
+    if (page >= 0) t.load(p.kp + at.at * (64 * D), p.vp + at.at * (64 * D), lane);
+    QueryTile<DC, PIECES> q[1];
+    take_queries<T, DC, PIECES>(q[0], query, there, p.scale, g);
+    for (int i = tile0 + wave; i < end; i += W) {
+      const int page1 = page_of(i + W);
+      if (page >= 0) {
+        const long k0 = 64L * range.at(i);
+        attend_tile<DC, PIECES, 1>(c, q, t, at.ks, at.vs, sees_whole(p, k0, cb.pos0, cb.pos1, sp.length), k0, pos, sp.length, p.window, p.keep, g);
+      }
+      page = page1;
+      at = tile_place(p, page, range.at(i + W), h);
+      if (page >= 0) t.load(p.kp + at.at * (64 * D), p.vp + at.at * (64 * D), lane);
     }
-    t = next;
-    at = at1;
-    page = page1;
-    page1 = page2;
-  }
 #pragma unroll
-  for (int i = 0; i < 4 * DC; ++i) *(f32x4*)&so[wave][lane & 15][16 * i + 4 * g] = c[0].o[i];
-  if (g == 0) { sm[wave][lane & 15] = c[0].m; sl[wave][lane & 15] = c[0].l[0]; }
-  __syncthreads();
-  // 16 threads per column
-  const int cc = threadIdx.x >> 4;
-  const int my = cb.first + cc;
-  if (my >= cb.end) return;
-  const int my_token = (unsigned)my / (unsigned)p.group, my_head = h * p.group + my - my_token * p.group;
-  float m = sm[0][cc];
+    for (int i = 0; i < 4 * DC; ++i) *(f32x4*)&so[wave][lane & 15][16 * i + 4 * g] = c[0].o[i];
+    if (g == 0) { sm[wave][lane & 15] = c[0].m; sl[wave][lane & 15] = c[0].l[0]; }
+    __syncthreads();
+    const int cc = threadIdx.x / (4 * W), in = threadIdx.x % (4 * W), my = cb.first + cc;  // 4 W threads per column
+    if (my < cb.end) {
+      float m = sm[0][cc];
 #pragma unroll
-  for (int w = 1; w < W; ++w) m = fmaxf(m, sm[w][cc]);
-  float f[W], sum = 0.f;
+      for (int w = 1; w < W; ++w) m = fmaxf(m, sm[w][cc]);
+      float f[W], sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < W; ++w) {
-    f[w] = __builtin_amdgcn_exp2f(sm[w][cc] - m);
-    sum += f[w] * sl[w][cc];
-  }
-  const long row = (long)(sp.row0 + my_token) * p.heads + my_head;
-  const float inv = p.part ? 1.f : (sum > 0.f || sum != sum ? 1.f / sum : 0.f);
-  float* part = p.part ? p.part + ((long)blockIdx.x * p.t.n_rows * p.heads + row) * (D + 4) : nullptr;
-  for (int d = 4 * (threadIdx.x & 15); d < D; d += 64) {
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < W; ++w) {
+        f[w] = __builtin_amdgcn_exp2f(sm[w][cc] - m);
+        sum += f[w] * sl[w][cc];
+      }
+      const int my_token = (unsigned)my / (unsigned)p.group, my_head = h * p.group + my - my_token * p.group;
+      const long row = (long)(sp.row0 + my_token) * p.heads + my_head;
+      const float inv = !all ? 1.f : (sum > 0.f || sum != sum ? 1.f / sum : 0.f);
+      // (a share cuts two units at most: the one it begins with and the one it ends with)
+      float* part = all ? nullptr : p.part + (((long)blockIdx.x * 2 + (done == share_begin ? 0 : 1)) * 16 + cc) * (D + 4);
+      for (int d = 4 * in; d < D; d += 16 * W) {
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < W; ++w) o += f[w] * *(const f32x4*)&so[w][cc][d];
-    o *= inv;
-    if (part) {
-      *(f32x4*)(part + d) = o;
-    } else {
-      *(u32x2*)(p.out + row * D + d) = u32x2{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])};
+        for (int w = 0; w < W; ++w) o += f[w] * *(const f32x4*)&so[w][cc][d];
+        o *= inv;
+        if (all) *(u32x2*)(p.out + row * D + d) = u32x2{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])};
+        else *(f32x4*)(part + d) = o;
+      }
+      if (!all && in == 0) { part[D] = m; part[D + 1] = sum; }
+    }
+    done += n;
+    if (!p.part || done >= share_end) return;
+    __syncthreads();
+    tile0 = 0;
+    if (++unit == work.blocks * p.kv_heads) {
+      unit = 0;
+      do ++b; while (uniform(before[b + 1]) <= done);  // (requests without new tokens)
+      sp = uniform(paged_span(p.t, b));
+      work = request_work(p, sp);
     }
   }
-  if (part && (threadIdx.x & 15) == 0) { part[D] = m; part[D + 1] = sum; }
+}
+
+// The units that shares have cut: a wave per row and head adds its parts up.
+template <typename T, int DC>
+__global__ void __launch_bounds__(256) paged_join_units_kernel(const PagedAttnParams p, int workgroups, int waves) {
+  constexpr int D = DC * 64;
+  const int lane = threadIdx.x & 63;
+  const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (item >= (long)p.t.n_rows * p.heads) return;
+  const int row = (int)(item / p.heads), head = (int)(item % p.heads);
+  const int b = request_of(p.t, row);
+  const PagedSpan sp = paged_span(p.t, b);
+  if (row < sp.row0 || row >= sp.row0 + sp.count) return;
+  const int col = (row - sp.row0) * p.group + head % p.group;
+  int blocks = (sp.count * p.group + 15) / 16;
+  blocks = blocks < p.col_tiles ? blocks : p.col_tiles;
+  if (col >= 16 * blocks) return;
+  const int first = p.before[b], tiles = (p.before[b + 1] - first) / (blocks * p.kv_heads);
+  const int begin = first + (col / 16 * p.kv_heads + head / p.group) * tiles;
+  const int share = share_of(p.before[p.t.n_requests], workgroups, waves);
+  const int w0 = begin / share, w1 = (begin + tiles - 1) / share;
+  if (w0 == w1) return;  // done by one
+  float m = kNoMax, sum = 0.f, o[DC] = {};
+  constexpr int kAtOnce = 4;
+  for (int w = w0; w <= w1; w += kAtOnce) {
+    float pm[kAtOnce], ps[kAtOnce], po[kAtOnce][DC];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int x = w + k <= w1 ? w + k : w1;
+      const float* part = p.part + (((long)x * 2 + (x * share >= begin ? 0 : 1)) * 16 + col % 16) * (D + 4);
+      pm[k] = part[D];
+      ps[k] = part[D + 1];
+#pragma unroll
+      for (int j = 0; j < DC; ++j) po[k][j] = part[64 * j + lane];
+    }
+    float to = m;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) to = fmaxf(to, pm[k]);
+    const float f0 = __builtin_amdgcn_exp2f(m - to);
+    m = to;
+    sum *= f0;
+#pragma unroll
+    for (int j = 0; j < DC; ++j) o[j] *= f0;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const float f = w + k <= w1 ? __builtin_amdgcn_exp2f(pm[k] - m) : 0.f;
+      sum += f * ps[k];
+#pragma unroll
+      for (int j = 0; j < DC; ++j) o[j] += w + k <= w1 ? f * po[k][j] : 0.f;
+    }
+  }
+  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+#pragma unroll
+  for (int j = 0; j < DC; ++j) p.out[item * D + 64 * j + lane] = T::pack(o[j] * inv);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -603,7 +759,7 @@ __global__ void __launch_bounds__(64 * W, W / 4 * (DC == 4 ? 1 : 2)) paged_tiles
     const bool there = col < cb.end;
     const unsigned at = there ? col : cb.end - 1, tok = at / (unsigned)p.group, head = at - tok * p.group;
     token[n] = there ? (int)tok : -1;
-    load_queries<T, DC, PIECES>(q[n], p.q + (long)(sp.row0 + (int)tok) * p.q_tok + (long)(h * p.group + (int)head) * p.q_head, there, p.scale, g);
+    take_queries<T, DC, PIECES>(q[n], request_queries<DC>(p.q + (long)(sp.row0 + (int)tok) * p.q_tok + (long)(h * p.group + (int)head) * p.q_head, g), there, p.scale, g);
 #pragma unroll
     for (int i = 0; i < 4 * DC; ++i) c[n].o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     c[n].l = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -791,15 +947,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (item >= n) return;
   const int row = (int)(item / p.heads), head = (int)(item % p.heads);
-  int b = row;
-  if (p.t.offsets) {
-    int lo = 0, hi = p.t.n_requests;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.t.offsets[mid] <= row) lo = mid; else hi = mid;
-    }
-    b = lo;
-  }
+  const int b = request_of(p.t, row);
   const PagedSpan sp = paged_span(p.t, b);
   if (row < sp.row0 || row >= sp.row0 + sp.count) return;
   const int col = (row - sp.row0) * p.group + head % p.group;
@@ -822,9 +970,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   for (int j = 0; j < DC; ++j) p.out[item * D + 64 * j + lane] = T::pack(o[j] * inv);
 }
 
-struct PagedPlan { int block_cols, col_tiles, split_tiles, splits; };
-static PagedPlan paged_plan(int n_requests, int max_tokens, int max_length, int window, int keep, int n_q_heads, int n_kv_heads, int head_dim) {
-  PagedPlan r;
+struct PagedPlan { int block_cols, col_tiles, split_tiles, splits, waves, workgroups; size_t scratch; };
+static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_length, int window, int keep, int n_q_heads, int n_kv_heads, int head_dim) {
+  PagedPlan r = {};
   const long group = n_q_heads / n_kv_heads;
   const bool prompt = max_tokens * group > 64;
   r.block_cols = prompt ? (head_dim == 256 ? 64 : 128) : 16;  // (256 dimensions: results of 32 columns a wave do not fit its registers)
@@ -835,12 +983,26 @@ static PagedPlan paged_plan(int n_requests, int max_tokens, int max_length, int 
     tiles = tiles < seen ? tiles : seen;
   }
   if (tiles < 1) tiles = 1;
-  const long work = (long)n_requests * n_kv_heads * r.col_tiles;
-  long splits = prompt ? (512 + work - 1) / work : (1024 + work - 1) / work;
-  if (splits > (tiles + 7) / 8) splits = (tiles + 7) / 8;
-  if (splits < 1) splits = 1;
-  r.split_tiles = (int)((tiles + splits - 1) / splits);
-  r.splits = (int)((tiles + r.split_tiles - 1) / r.split_tiles);
+  const long units = (long)n_requests * n_kv_heads * r.col_tiles;
+  r.splits = 1;
+  r.split_tiles = (int)tiles;
+  if (prompt) {
+    long splits = (512 + units - 1) / units;
+    if (splits > (tiles + 7) / 8) splits = (tiles + 7) / 8;
+    if (splits < 1) splits = 1;
+    r.split_tiles = (int)((tiles + splits - 1) / splits);
+    r.splits = (int)((tiles + r.split_tiles - 1) / r.split_tiles);
+    r.scratch = r.splits > 1 ? (size_t)r.splits * n_rows * n_q_heads * (head_dim + 4) * 4 : 0;
+    return r;
+  }
+  // Eight waves to a workgroup and one workgroup to a CU, or four and two: eight cut fewer units, four have more of them at work where the shares are small. us, four / eight:
+  // 64 heads x 64 dimensions, 16 requests of 4096 keys 27.7 / 22.0; 128 dimensions, 32 requests of 200 to 4096 keys 35.5 / 40.7, 64 of 4096 to 16384 195.6 / 190.7.
+  // 256 dimensions: a wave's registers are all of a SIMD's.
+  r.waves = head_dim == 256 ? 4 : head_dim == 64 || tiles <= 16 || units * tiles >= 128 * 256 ? 8 : 4;
+  if (tiles <= 16 || n_requests > kDealtRequests || units * tiles > 0x3fffffffL) return r;  // a workgroup per unit
+  const long wanted = (units * tiles + r.waves - 1) / r.waves, most = head_dim == 256 || r.waves == 8 ? 256 : 512;
+  r.workgroups = (int)(wanted < most ? wanted : most);
+  r.scratch = (((size_t)n_requests + 1) * 4 + 255) / 256 * 256 + (size_t)r.workgroups * 2 * 16 * (head_dim + 4) * 4;
   return r;
 }
 
@@ -856,8 +1018,7 @@ static bool paged_attention_sizes(int n_rows, int n_requests, int max_tokens, in
 extern "C" size_t mui_paged_attention_scratch_bytes(int n_rows, int n_requests, int max_tokens, int max_length, int window, int keep_first, int n_q_heads,
                                                     int n_kv_heads, int head_dim) {
   if (!paged_attention_sizes(n_rows, n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads, head_dim)) return 0;
-  const PagedPlan plan = paged_plan(n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads, head_dim);
-  return plan.splits > 1 ? (size_t)plan.splits * n_rows * n_q_heads * (head_dim + 4) * 4 : 0;
+  return paged_plan(n_rows, n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads, head_dim).scratch;
 }
 
 extern "C" int mui_paged_attention(mui_stream_t stream, int dtype, const void* q, long q_token_stride, long q_head_stride, const void* k_pages,
@@ -875,12 +1036,12 @@ extern "C" int mui_paged_attention(mui_stream_t stream, int dtype, const void* q
   if ((q_token_stride | q_head_stride) & 7) return MUI_ERR_ALIGNMENT;
   const long cap = (long)table_pages * page_tokens;
   if (max_length > cap) max_length = (int)cap;
-  const PagedPlan plan = paged_plan(n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads, head_dim);
-  if (plan.splits > 1 && (!scratch || scratch_bytes < (size_t)plan.splits * n_rows * n_q_heads * (head_dim + 4) * 4)) return MUI_ERR_INVALID_ARG;
+  const PagedPlan plan = paged_plan(n_rows, n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads, head_dim);
+  if (plan.scratch && (!scratch || scratch_bytes < plan.scratch)) return MUI_ERR_INVALID_ARG;
   if ((long)n_rows * n_q_heads > 0x7fffffffL - 256) return MUI_ERR_UNSUPPORTED;
   const bool prompt = plan.block_cols > 16;
   const long blocks = (long)plan.col_tiles * n_kv_heads * n_requests;
-  if (blocks > 0x7fffffffL || plan.splits > 65535 || n_requests > 65535 || (!prompt && (long)plan.col_tiles * n_kv_heads > 65535)) return MUI_ERR_UNSUPPORTED;
+  if (blocks > 0x7fffffffL || plan.splits > 65535 || n_requests > 65535) return MUI_ERR_UNSUPPORTED;
   PagedAttnParams p = {};
   p.q = (const uint16_t*)q; p.q_tok = q_token_stride; p.q_head = q_head_stride;
   p.kp = (const uint8_t*)k_pages; p.vp = (const uint8_t*)v_pages; p.ks = k_scale; p.vs = v_scale;
@@ -889,18 +1050,31 @@ extern "C" int mui_paged_attention(mui_stream_t stream, int dtype, const void* q
   p.window = window; p.keep = window > 0 ? keep_first : 0;
   p.heads = n_q_heads; p.kv_heads = n_kv_heads; p.group = n_q_heads / n_kv_heads;
   p.block_cols = plan.block_cols; p.col_tiles = plan.col_tiles; p.split_tiles = plan.split_tiles; p.splits = plan.splits;
-  p.part = plan.splits > 1 ? (float*)scratch : nullptr;
+  if (plan.scratch && prompt) p.part = (float*)scratch;
+  if (plan.scratch && !prompt) {
+    p.before = (int*)scratch;
+    p.part = (float*)((char*)scratch + (((size_t)n_requests + 1) * 4 + 255) / 256 * 256);
+  }
   p.out = (uint16_t*)out;
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid(plan.splits, plan.col_tiles * n_kv_heads, n_requests);
+  const dim3 grid((unsigned)(plan.workgroups ? plan.workgroups : blocks));
   const dim3 join((unsigned)(((long)n_rows * n_q_heads + 3) / 4));
-#define MUI_PAGED_GO(TT, DC, PIECES)                                                                     \
-  do {                                                                                                   \
-    if (prompt)                                                                                          \
+#define MUI_PAGED_GO(TT, DC, PIECES)                                                                                                       \
+  do {                                                                                                                                     \
+    if (prompt) {                                                                                                                          \
       hipLaunchKernelGGL((paged_tiles_kernel<TT, DC, PIECES, DC == 4 ? 1 : 2, 4>), dim3((unsigned)blocks, plan.splits), dim3(256), 0, s, p); \
-    else                                                                                                 \
-      hipLaunchKernelGGL((paged_columns_kernel<TT, DC, PIECES>), grid, dim3(256), 0, s, p);              \
-    if (plan.splits > 1) hipLaunchKernelGGL((paged_join_kernel<TT, DC>), join, dim3(256), 0, s, p);      \
+      if (p.part) hipLaunchKernelGGL((paged_join_kernel<TT, DC>), join, dim3(256), 0, s, p);                                               \
+    } else {                                                                                                                               \
+      if constexpr (DC < 4) {                                                                                                              \
+        if (plan.waves == 8)                                                                                                               \
+          hipLaunchKernelGGL((paged_columns_kernel<TT, DC, PIECES, 8>), grid, dim3(512), 0, s, p);                                         \
+      }                                                                                                                                    \
+      if constexpr (DC > 1) {                                                                                                              \
+        if (plan.waves == 4)                                                                                                               \
+          hipLaunchKernelGGL((paged_columns_kernel<TT, DC, PIECES, 4>), grid, dim3(256), 0, s, p);                                         \
+      }                                                                                                                                    \
+      if (p.part) hipLaunchKernelGGL((paged_join_units_kernel<TT, DC>), join, dim3(256), 0, s, p, plan.workgroups, plan.waves);            \
+    }                                                                                                                                      \
   } while (0)
 #define MUI_PAGED_TYPES(DC) \
   do { if (dtype == MUI_DTYPE_F16) MUI_PAGED_GO(F16, DC, 3); else MUI_PAGED_GO(BF16, DC, 2); } while (0)
