@@ -40,6 +40,24 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedTable& p, int b) {
   return s;
 }
 
+// the last request whose rows begin at or before `row`
+__device__ __forceinline__ int request_of(const PagedTable& t, int row) {
+  if (!t.offsets) return row;
+  int lo = 0, hi = t.n_requests;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.offsets[mid] <= row) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// (what a request's numbers say is the same for a workgroup, which the compiler does not see where they come from memory: in scalar registers it costs the results no room)
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long uniform(long x) {
+  return (long)((unsigned long long)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)(x & 0xffffffffL)));
+}
+__device__ __forceinline__ PagedSpan uniform(PagedSpan s) { return {uniform(s.row0), uniform(s.count), uniform(s.start), uniform(s.length)}; }
+
 // the page of slot `slot` of request b's table, or -1 where that is none
 __device__ __forceinline__ int paged_page(const PagedTable& p, int b, int slot) {
   const int page = slot < p.pages ? p.table[(long)b * p.stride + slot] : -1;

@@ -5,7 +5,8 @@
 // type; keys and values once, to codes x / scale. The scale of a page and head is the smallest power of two with which the largest new
 // value fits 448, but not below what stands there for the page's earlier tokens; where it grows their codes follow.
 //
-// A thread works on units of 16 dimensions, which hold their pairs whole: 8 + 8 at a distance of rot / 2, or 16 in a row.
+// A thread works on units of two chunks of 8 dimensions, which hold their pairs whole: pairs of halves lie rot / 2 apart, and so do the chunks; of interleaved pairs and of
+// dimensions that do not turn unit u has chunks u and u + half of them, so that neighbours' loads are neighbours too.
 #include "paged.cuh"
 
 namespace mui {
@@ -22,47 +23,63 @@ struct AppendParams {
   PagedTable t;
   float rope_scale;
   int rot, interleaved, heads, kv_heads, dim;
-  int q_blocks, spans;
+  int q_blocks, at_once;  // at_once: KV heads of a workgroup
 };
 
-// dimension of the first value of either half of a unit
-__device__ __forceinline__ void unit_dims(const AppendParams& p, int u, bool turned, int& d0, int& d1) {
-  if (turned && !p.interleaved) {
-    d0 = 8 * u;
-    d1 = d0 + (p.rot >> 1);
-  } else {
-    d0 = 16 * u;
-    d1 = d0 + 8;
+// A unit: first dimensions of its chunks, and which of them turn.
+struct Unit { int d0, d1; bool turns0, turns1; };
+__device__ __forceinline__ Unit unit_of(const AppendParams& p, int u) {
+  const int units = p.dim >> 4, turned = p.rot >> 4;
+  if (p.interleaved) return {8 * u, 8 * (u + units), 8 * u < p.rot, 8 * (u + units) < p.rot};
+  if (u < turned) return {8 * u, 8 * u + (p.rot >> 1), true, true};
+  return {p.rot + 8 * (u - turned), p.rot + 8 * (u - turned + units - turned), false, false};
+}
+
+// The angles of its eight pairs: halves 8 u .. 8 u + 7; interleaved four of either chunk. Those of a chunk that does not turn are not used.
+__device__ __forceinline__ void unit_angles(const AppendParams& p, const Unit& n, double pos, float (&c)[8], float (&s)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (!(i < 4 ? n.turns0 : n.turns1)) continue;
+    const int pair = !p.interleaved ? n.d0 + i : i < 4 ? (n.d0 >> 1) + i : (n.d1 >> 1) + i - 4;
+    // the turns left over in 32 bits, and what that rounding took from them (it is 3 of the last places of a sine: enough to move a code in a few thousand)
+    double a = pos * p.inv_freq[pair] * 0.15915494309189533576888376337251;
+    a = 2.0 * (a - rint(a));
+    const float f = (float)a, r = 3.14159265f * (float)(a - (double)f);
+    float cf, sf;
+    sincospif(f, &sf, &cf);
+    c[i] = p.rope_scale * fmaf(-r, sf, cf);
+    s[i] = p.rope_scale * fmaf(r, cf, sf);
   }
 }
 
-__device__ __forceinline__ void unit_angles(const AppendParams& p, int u, double pos, float (&c)[8], float (&s)[8]) {
+// x: the values of the two chunks
+__device__ __forceinline__ void unit_turn(const AppendParams& p, const Unit& n, const float (&c)[8], const float (&s)[8], float (&x)[16]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    rope_angle(pos, p.inv_freq[8 * u + i], c[i], s[i]);
-    c[i] *= p.rope_scale;
-    s[i] *= p.rope_scale;
-  }
-}
-
-// x: 16 values of a unit in the order of its two halves
-__device__ __forceinline__ void unit_turn(bool interleaved, const float (&c)[8], const float (&s)[8], float (&x)[16]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int ia = interleaved ? 2 * i : i, ib = interleaved ? 2 * i + 1 : i + 8;
-    const float a = x[ia], b = x[ib];
-    x[ia] = a * c[i] - b * s[i];
-    x[ib] = b * c[i] + a * s[i];
+    if (!(i < 4 ? n.turns0 : n.turns1)) continue;
+    if (p.interleaved) {
+      const float a = x[2 * i], b = x[2 * i + 1];
+      x[2 * i] = a * c[i] - b * s[i];
+      x[2 * i + 1] = b * c[i] + a * s[i];
+    } else {
+      const float a = x[i], b = x[i + 8];
+      x[i] = a * c[i] - b * s[i];
+      x[i + 8] = b * c[i] + a * s[i];
+    }
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void load_unit(const uint16_t* row, int d0, int d1, float (&x)[16]) {
+__device__ __forceinline__ void unpack_unit(const u32x4 v, const u32x4 w, float (&x)[16]) {
   float a[8], b[8];
-  unpack8<T>(ld16(row + d0), a);
-  unpack8<T>(ld16(row + d1), b);
+  unpack8<T>(v, a);
+  unpack8<T>(w, b);
 #pragma unroll
   for (int i = 0; i < 8; ++i) { x[i] = a[i]; x[8 + i] = b[i]; }
+}
+template <typename T>
+__device__ __forceinline__ void load_unit(const uint16_t* row, int d0, int d1, float (&x)[16]) {
+  unpack_unit<T>(ld16(row + d0), ld16(row + d1), x);
 }
 template <typename T>
 __device__ __forceinline__ void store_unit(uint16_t* row, int d0, int d1, const float (&x)[16]) {
@@ -132,15 +149,14 @@ __global__ void __launch_bounds__(256) append_step_kernel(const AppendParams p) 
   h -= kind == 0 ? 0 : (kind == 1 ? p.heads : p.heads + p.kv_heads);
   const uint16_t* row = kind == 0 ? p.q + (long)sp.row0 * p.q_tok + (long)h * p.q_head
                         : kind == 1 ? p.k + (long)sp.row0 * p.k_tok + (long)h * p.k_head : p.v + (long)sp.row0 * p.v_tok + (long)h * p.v_head;
-  const bool turned = kind != 2 && 16 * u < p.rot;
-  int d0, d1;
-  unit_dims(p, u, turned, d0, d1);
+  const Unit n = unit_of(p, u);
+  const int d0 = n.d0, d1 = n.d1;
   float x[16];
   load_unit<T>(row, d0, d1, x);
-  if (turned) {
+  if (kind != 2 && n.turns0) {  // (the second chunk turns only where the first does)
     float c[8], s[8];
-    unit_angles(p, u, (double)(p.positions ? p.positions[sp.row0] : sp.start), c, s);
-    unit_turn(p.interleaved, c, s, x);
+    unit_angles(p, n, (double)(p.positions ? p.positions[sp.row0] : sp.start), c, s);
+    unit_turn(p, n, c, s, x);
   }
   if (kind == 0) {
     store_unit<T>(p.q_out + ((long)sp.row0 * p.heads + h) * p.dim, d0, d1, x);
@@ -183,113 +199,219 @@ __global__ void __launch_bounds__(256) append_step_kernel(const AppendParams p) 
 }
 
 // ---------------------------------------------------------------------------------------
-// prompts: workgroups of queries (16 tokens each), then one workgroup per page, head and kind
+// prompts: workgroups of queries, then one per page, head and kind
 // ---------------------------------------------------------------------------------------
+constexpr int kQueryHeads = 8;  // of a workgroup: its angles serve that many, four loads at a time
+
 template <typename T>
-__global__ void __launch_bounds__(256) append_rows_kernel(const AppendParams p) {
-  const int units = p.dim >> 4;
-  __shared__ float red[4];
+__device__ __forceinline__ void append_queries(const AppendParams& p, int block) {
+  const int units = p.dim >> 4, per = (int)blockDim.x / units;  // tokens of a workgroup
+  const int groups = (p.heads + kQueryHeads - 1) / kQueryHeads;
+  const int h0 = block % groups * kQueryHeads, h1 = h0 + kQueryHeads < p.heads ? h0 + kQueryHeads : p.heads;
+  const int u = threadIdx.x % units;
+  const int row = block / groups * per + threadIdx.x / units;
+  if (row >= p.t.n_rows) return;
+  const Unit n = unit_of(p, u);
+  constexpr int kAhead = 4;
+  u32x4 raw[kAhead][2];
+  auto request = [&](int h) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const uint16_t* from = p.q + (long)row * p.q_tok + (long)(h + k < h1 ? h + k : h1 - 1) * p.q_head;
+      raw[k][0] = ld16(from + n.d0);
+      raw[k][1] = ld16(from + n.d1);
+    }
+  };
+  request(h0);  // (on their way while the row's place is looked up)
+  const int b = request_of(p.t, row);
+  if (b >= p.t.n_requests) return;
+  const PagedSpan sp = paged_span(p.t, b);
+  if (row < sp.row0 || row >= sp.row0 + sp.count) return;  // behind the last request: left as it is
+  float c[8], s[8];
+  if (n.turns0) unit_angles(p, n, (double)(p.positions ? p.positions[row] : sp.start + (row - sp.row0)), c, s);
+  for (int h = h0; h < h1; h += kAhead) {
+    float x[kAhead][16];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) unpack_unit<T>(raw[k][0], raw[k][1], x[k]);
+    if (h + kAhead < h1) request(h + kAhead);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (h + k >= h1) break;
+      if (n.turns0) unit_turn(p, n, c, s, x[k]);
+      store_unit<T>(p.q_out + ((long)row * p.heads + h + k) * p.dim, n.d0, n.d1, x[k]);
+    }
+  }
+}
+
+// the largest of `most` over the workgroup
+__device__ __forceinline__ float block_most(float most, float* red) {
+  most = wave_max(most);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
+  __syncthreads();
+  for (int w = 0; w < (int)blockDim.x / kWave; ++w) most = fmaxf(most, red[w]);
+  return most;
+}
+
+// The new exponent of a page and head that holds `old` earlier tokens, whose codes follow where it rises.
+__device__ __forceinline__ int page_exponent(const AppendParams& p, float most, uint8_t* base, float* scale, float before_s, int old, bool values) {
+  int e = e4m3_exponent(most);
+  if (old > 0) {
+    const int before = scale_exponent(before_s);
+    if (e > before) {
+      const int down = before - e;
+      move_codes(base, p.dim, old, exp2i(down < -126 ? -126 : down), values, threadIdx.x, blockDim.x);
+      __syncthreads();  // (a new value's bytes may lie between moved ones)
+    } else {
+      e = before;
+    }
+  }
+  if (threadIdx.x == 0) *scale = exp2i(e);
+  return e;
+}
+
+// A page of a head is 32 values a thread (64 and 128 of the larger ones), which it holds between finding the largest and writing the codes. Keys: units of a token, as queries.
+// Values: 8 dimensions of four tokens 4 q .. 4 q + 3, whose codes are a dword of each dimension's row. A workgroup takes the keys or the
+// values of several heads where there are many pages: workgroups begin no faster than about 130 a microsecond, and keys' angles serve them all.
+template <typename T, int IT>
+__global__ void __launch_bounds__(512) append_rows_kernel(const AppendParams p) {
+  __shared__ float red[16];
   if ((int)blockIdx.x < p.q_blocks) {
-    const int per = 256 / units;  // tokens of a workgroup
-    const int u = threadIdx.x % units;
-    const int row = blockIdx.x * per + threadIdx.x / units;
-    if (row >= p.t.n_rows) return;
-    int b = row;
-    if (p.t.offsets) {  // the last request that starts at or before the row
-      int lo = 0, hi = p.t.n_requests;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.t.offsets[mid] <= row) lo = mid; else hi = mid;
-      }
-      b = lo;
-    }
-    if (b >= p.t.n_requests) return;
-    const PagedSpan sp = paged_span(p.t, b);
-    if (row < sp.row0 || row >= sp.row0 + sp.count) return;  // behind the last request: left as it is
-    const bool turned = 16 * u < p.rot;
-    int d0, d1;
-    unit_dims(p, u, turned, d0, d1);
-    float c[8], s[8];
-    if (turned) unit_angles(p, u, (double)(p.positions ? p.positions[row] : sp.start + (row - sp.row0)), c, s);
-    for (int h = 0; h < p.heads; ++h) {
-      float x[16];
-      load_unit<T>(p.q + (long)row * p.q_tok + (long)h * p.q_head, d0, d1, x);
-      if (turned) unit_turn(p.interleaved, c, s, x);
-      store_unit<T>(p.q_out + ((long)row * p.heads + h) * p.dim, d0, d1, x);
-    }
+    append_queries<T>(p, blockIdx.x);
     return;
   }
   int i = blockIdx.x - p.q_blocks;
-  const int hk = i % (2 * p.kv_heads);
-  i /= 2 * p.kv_heads;
-  const int span = i % p.spans, b = i / p.spans;
-  const bool values = hk >= p.kv_heads;
-  const int h = values ? hk - p.kv_heads : hk;
-  const PagedSpan sp = paged_span(p.t, b);
-  const int P = 1 << p.t.page_shift;
+  const int groups = (p.kv_heads + p.at_once - 1) / p.at_once;
+  const bool values = i % (2 * groups) >= groups;
+  const int h0 = i % groups * p.at_once, h1 = h0 + p.at_once < p.kv_heads ? h0 + p.at_once : p.kv_heads;
+  i /= 2 * groups;
+  const int P = 1 << p.t.page_shift, units = p.dim >> 4, threads = blockDim.x;
+  // the i-th page that takes new tokens: every wave adds the requests' pages up, 64 at a time
+  int b = -1;
+  long slot = 0;
+  for (int r0 = 0; r0 < p.t.n_requests && b < 0; r0 += kWave) {
+    const int r = r0 + (threadIdx.x & 63);
+    int pages = 0;
+    long from = 0;
+    if (r < p.t.n_requests) {
+      const PagedSpan s = paged_span(p.t, r);
+      from = (s.start < 0 ? 0 : s.start) >> p.t.page_shift;
+      if (s.count > 0 && s.length > 0 && ((s.length - 1) >> p.t.page_shift) >= from) pages = (int)(((s.length - 1) >> p.t.page_shift) - from) + 1;
+    }
+    int to = pages;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(to, off);
+      if ((int)(threadIdx.x & 63) >= off) to += o;
+    }
+    const unsigned long long in = __ballot(to > i);
+    if (in) {
+      const int l = __ffsll((long long)in) - 1;
+      b = uniform(r0 + l);
+      slot = uniform(__shfl((int)from, l) + i - __shfl(to - pages, l));
+    } else {
+      i -= __shfl(to, 63);
+    }
+  }
+  if (b < 0) return;
+  const PagedSpan sp = uniform(paged_span(p.t, b));
   const long first = sp.start < 0 ? 0 : sp.start;
-  for (long slot = (first >> p.t.page_shift) + span; slot * P < sp.length; slot += p.spans) {
+  {
     const int page = paged_page(p.t, b, (int)slot);
-    if (page < 0) continue;
+    if (page < 0) return;
     const long low = first > slot * P ? first : slot * P;
     const long end = sp.length < (slot + 1) * P ? sp.length : (slot + 1) * P;
-    const int n = (int)(end - low), at0 = (int)(low - slot * P);
-    if (n <= 0) continue;
-    const int row0 = sp.row0 + (int)(low - sp.start);
-    const long ph = (long)page * p.kv_heads + h;
-    uint8_t* base = (values ? p.vp : p.kp) + ph * ((long)p.dim << p.t.page_shift);
-    float* scale = (values ? p.vs : p.ks) + ph;
-    const float before_s = *scale;
-    float most = 0.f;
-    float inv = 0.f;
-    for (int pass = 0; pass < 2; ++pass) {  // the largest value, then the codes
-      for (int j = threadIdx.x; j < n * units; j += 256) {
-        const int u = j % units, row = row0 + j / units, at = at0 + j / units;
-        const bool turned = !values && 16 * u < p.rot;
-        int d0, d1;
-        unit_dims(p, u, turned, d0, d1);
-        float x[16];
-        load_unit<T>(values ? p.v + (long)row * p.v_tok + (long)h * p.v_head : p.k + (long)row * p.k_tok + (long)h * p.k_head, d0, d1, x);
-        if (turned) {
-          float c[8], s[8];
-          unit_angles(p, u, (double)(p.positions ? p.positions[row] : sp.start + (row - sp.row0)), c, s);
-          unit_turn(p.interleaved, c, s, x);
+    const int at0 = (int)(low - slot * P), at1 = (int)(end - slot * P);
+    if (at1 <= at0) return;
+    const int row0 = sp.row0 + (int)(low - sp.start) - at0;  // of the page's first place
+    if (!values) {
+      constexpr bool kHeld = IT == 1;  // angles for all heads (of a larger page there are too many to hold)
+      float c[kHeld ? 2 : 1][8], s[kHeld ? 2 : 1][8];
+#pragma unroll
+      for (int k = 0; k < (kHeld ? 2 : 0); ++k) {
+        const int j = threadIdx.x + k * threads, u = j % units, at = j / units;
+        const Unit n = unit_of(p, u);
+        if (at >= at0 && at < at1 && n.turns0) unit_angles(p, n, (double)(p.positions ? p.positions[row0 + at] : slot * P + at), c[k], s[k]);
+      }
+      for (int h = h0; h < h1; ++h) {
+        const long ph = (long)page * p.kv_heads + h;
+        uint8_t* base = p.kp + ph * ((long)p.dim << p.t.page_shift);
+        const float before_s = p.ks[ph];
+        float most = 0.f, x[2 * IT][16];
+#pragma unroll
+        for (int k = 0; k < 2 * IT; ++k) {
+          const int j = threadIdx.x + k * threads, u = j % units, at = j / units;
+          if (at >= at0 && at < at1) {
+            const Unit n = unit_of(p, u);
+            load_unit<T>(p.k + (long)(row0 + at) * p.k_tok + (long)h * p.k_head, n.d0, n.d1, x[k]);
+            if (n.turns0) {
+              if constexpr (!kHeld) unit_angles(p, n, (double)(p.positions ? p.positions[row0 + at] : slot * P + at), c[0], s[0]);
+              unit_turn(p, n, c[kHeld ? k : 0], s[kHeld ? k : 0], x[k]);
+            }
+#pragma unroll
+            for (int m = 0; m < 16; ++m) most = fmaxf(most, finite_abs(x[k][m]));
+          }
         }
-        if (pass == 0) {
+        __syncthreads();  // (red)
+        const float inv = exp2i(-page_exponent(p, block_most(most, red), base, p.ks + ph, before_s, at0, false));
 #pragma unroll
-          for (int k = 0; k < 16; ++k) most = fmaxf(most, finite_abs(x[k]));
-        } else {
-          uint32_t w[4];
+        for (int k = 0; k < 2 * IT; ++k) {
+          const int j = threadIdx.x + k * threads, u = j % units, at = j / units;
+          if (at >= at0 && at < at1) {
+            const Unit n = unit_of(p, u);
+            uint32_t w[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = to_e4m3x4(x[4 * k] * inv, x[4 * k + 1] * inv, x[4 * k + 2] * inv, x[4 * k + 3] * inv);
-          if (!values) {
-            *(u32x2*)(base + k_at(p.dim, at, d0)) = u32x2{w[0], w[1]};
-            *(u32x2*)(base + k_at(p.dim, at, d1)) = u32x2{w[2], w[3]};
-          } else {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) base[v_at(p.dim, at, (k < 8 ? d0 : d1 - 8) + k)] = (uint8_t)(w[k >> 2] >> (8 * (k & 3)));
+            for (int m = 0; m < 4; ++m) w[m] = to_e4m3x4(x[k][4 * m] * inv, x[k][4 * m + 1] * inv, x[k][4 * m + 2] * inv, x[k][4 * m + 3] * inv);
+            *(u32x2*)(base + k_at(p.dim, at, n.d0)) = u32x2{w[0], w[1]};
+            *(u32x2*)(base + k_at(p.dim, at, n.d1)) = u32x2{w[2], w[3]};
           }
         }
       }
-      if (pass) break;
-      most = wave_max(most);
-      __syncthreads();
-      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
-      __syncthreads();
-      most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-      int e = e4m3_exponent(most);
-      if (at0 > 0) {
-        const int before = scale_exponent(before_s);
-        if (e > before) {
-          const int down = before - e;
-          move_codes(base, p.dim, at0, exp2i(down < -126 ? -126 : down), values, threadIdx.x, 256);
-          __syncthreads();  // (a new value's byte may lie between moved ones)
-        } else {
-          e = before;
+      return;
+    }
+    for (int h = h0; h < h1; ++h) {
+      const long ph = (long)page * p.kv_heads + h;
+      uint8_t* base = p.vp + ph * ((long)p.dim << p.t.page_shift);
+      const float before_s = p.vs[ph];
+      float most = 0.f;
+      u32x4 raw[IT][4];
+#pragma unroll
+      for (int k = 0; k < IT; ++k) {
+        const int j = threadIdx.x + k * threads, d0 = (j & 7) * 8 + (j / (2 * P)) * 64, quad = j / 8 % (P / 4);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const int at = 4 * quad + m;
+          raw[k][m] = u32x4{0, 0, 0, 0};
+          if (at >= at0 && at < at1) raw[k][m] = ld16(p.v + (long)(row0 + at) * p.v_tok + (long)h * p.v_head + d0);
         }
       }
-      if (threadIdx.x == 0) *scale = exp2i(e);
-      inv = exp2i(-e);
+#pragma unroll
+      for (int k = 0; k < IT; ++k)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          float x[8];
+          unpack8<T>(raw[k][m], x);
+#pragma unroll
+          for (int d = 0; d < 8; ++d) most = fmaxf(most, finite_abs(x[d]));
+        }
+      __syncthreads();  // (red)
+      const float inv = exp2i(-page_exponent(p, block_most(most, red), base, p.vs + ph, before_s, at0, true));
+#pragma unroll
+      for (int k = 0; k < IT; ++k) {
+        const int j = threadIdx.x + k * threads, d0 = (j & 7) * 8 + (j / (2 * P)) * 64, quad = j / 8 % (P / 4);
+        const int before = at0 - 4 * quad, behind = 4 * quad + 4 - at1;  // places of the four that stay as they are
+        if (before >= 4 || behind >= 4) continue;
+        float x[4][8];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) unpack8<T>(raw[k][m], x[m]);
+        const uint32_t keep = (before > 0 ? (1u << (8 * before)) - 1u : 0u) | (behind > 0 ? ~(0xffffffffu >> (8 * behind)) : 0u);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          uint32_t* to = (uint32_t*)(base + v_at(p.dim, 4 * quad, d0 + d));
+          uint32_t w = to_e4m3x4(x[0][d] * inv, x[1][d] * inv, x[2][d] * inv, x[3][d] * inv);
+          if (keep) w = (w & ~keep) | (*to & keep);
+          *to = w;
+        }
+      }
     }
   }
 }
@@ -334,13 +456,22 @@ extern "C" int mui_paged_append(mui_stream_t stream, int dtype, const void* q, l
       hipLaunchKernelGGL((append_step_kernel<BF16>), dim3((unsigned)blocks), dim3(256), 0, s, p);
     return launch_status();
   }
-  p.q_blocks = q ? (n_rows + 256 / units - 1) / (256 / units) : 0;
-  p.spans = (max_tokens + page_tokens - 2) / page_tokens + 1;
-  const long blocks = p.q_blocks + (long)n_requests * p.spans * 2 * n_kv_heads;
+  // 32 values a thread, of the larger pages 64 and 128
+  const int values = page_tokens * head_dim / 32, threads = values < 512 ? values : 512;
+  const long rows_per = threads / units;
+  const long q_blocks = q ? (n_rows + rows_per - 1) / rows_per * ((n_q_heads + kQueryHeads - 1) / kQueryHeads) : 0;
+  const long pages = (long)n_rows / page_tokens + 2 * (long)n_requests;  // that new tokens can lie in
+  p.at_once = pages * 2 * n_kv_heads > 1024 ? 2 : 1;
+  const long blocks = q_blocks + pages * 2 * ((n_kv_heads + p.at_once - 1) / p.at_once);
   if (blocks > 0x7fffffffL) return MUI_ERR_UNSUPPORTED;
-  if (dtype == MUI_DTYPE_F16)
-    hipLaunchKernelGGL((append_rows_kernel<F16>), dim3((unsigned)blocks), dim3(256), 0, s, p);
-  else
-    hipLaunchKernelGGL((append_rows_kernel<BF16>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+  p.q_blocks = (int)q_blocks;
+  const dim3 grid((unsigned)blocks), block(threads);
+#define MUI_APPEND_GO(TT)                                                                             \
+  do {                                                                                                \
+    if (values <= 512) hipLaunchKernelGGL((append_rows_kernel<TT, 1>), grid, block, 0, s, p);         \
+    else if (values == 1024) hipLaunchKernelGGL((append_rows_kernel<TT, 2>), grid, block, 0, s, p);   \
+    else hipLaunchKernelGGL((append_rows_kernel<TT, 4>), grid, block, 0, s, p);                       \
+  } while (0)
+  if (dtype == MUI_DTYPE_F16) MUI_APPEND_GO(F16); else MUI_APPEND_GO(BF16);
   return launch_status();
 }

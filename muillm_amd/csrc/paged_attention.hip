@@ -2,7 +2,7 @@
 //
 // The matrix cores take the codes as they lie in memory: v_mfma_scale_f32_16x16x128_f8f6f4, whose block exponents carry the pages' scales. What
 // meets them is split into pieces of e4m3 so that nothing is lost by it: a query into two (bf16: 8 bits are two pieces of 4) or three (fp16), each 2^5 below
-// the one before; a probability into two, of 8 bits together, relative to the largest of its query's 64 in the tile (2^-18 of it at least), which goes
+// the one before; a probability into two (fp16: three), of 8 (12) bits together, relative to the largest of its query's 64 in the tile (2^-18 of it at least), which goes
 // with the product as its block exponent -- so a tile whose keys weigh little is as exact as one whose weigh much, however long the cache.
 // Sums and the running maximum are 32 bits; the maximum is rounded up to a whole power of two, so moving to a new one is exact.
 //
@@ -38,24 +38,6 @@ __device__ __forceinline__ int share_of(int total, int workgroups, int waves) {
   const int s = (total + workgroups - 1) / workgroups;
   return s > waves ? s : waves;
 }
-
-// the last request whose rows begin at or before `row`
-__device__ __forceinline__ int request_of(const PagedTable& t, int row) {
-  if (!t.offsets) return row;
-  int lo = 0, hi = t.n_requests;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (t.offsets[mid] <= row) lo = mid; else hi = mid;
-  }
-  return lo;
-}
-
-// (what a request's numbers say is the same for a workgroup, which the compiler does not see where they come from memory: in scalar registers it costs the results no room)
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ long uniform(long x) {
-  return (long)((unsigned long long)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)(x & 0xffffffffL)));
-}
-__device__ __forceinline__ PagedSpan uniform(PagedSpan s) { return {uniform(s.row0), uniform(s.count), uniform(s.start), uniform(s.length)}; }
 
 // The tiles of 64 keys that queries at positions first .. last see: `kept` from the beginning, then those from `from` to `end`.
 struct TileRange { int kept, from, end; __device__ int count() const { return kept + (end > from ? end - from : 0); }
@@ -211,7 +193,7 @@ __device__ __forceinline__ void attend_tile(Columns<DC> (&c)[NT], const QueryTil
         for (int j = 0; j < PIECES; ++j) s[n][i] = mfma_e4m3(kk, q[n].piece[j][m], s[n][i], 127, 127 - 5 * j);
     }
   }
-  i32x8 pp[NT];
+  i32x8 pp[NT], rest[NT];  // rest: fp16's third pieces, each 2^5 below what it adds to; the same values of the cache twice as in pp, the second time times zero
   int sb[NT];
   uint32_t seen[NT];  // keys 16 i + 4 g + r: bit 4 i + r
 #pragma unroll
@@ -249,7 +231,14 @@ __device__ __forceinline__ void attend_tile(Columns<DC> (&c)[NT], const QueryTil
       const uint32_t hi = to_e4m3x4(e[0], e[1], e[2], e[3]);
       const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true);
       pp[n][i] = (int)hi;
-      pp[n][4 + i] = (int)to_e4m3x4(e[0] - a[0], e[1] - a[1], e[2] - b[0], e[3] - b[1]);
+      const float d[4] = {e[0] - a[0], e[1] - a[1], e[2] - b[0], e[3] - b[1]};
+      const uint32_t lo = to_e4m3x4(d[0], d[1], d[2], d[3]);
+      pp[n][4 + i] = (int)lo;
+      if constexpr (PIECES == 3) {
+        const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, false), y = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, true);
+        rest[n][i] = (int)to_e4m3x4(32.f * (d[0] - x[0]), 32.f * (d[1] - x[1]), 32.f * (d[2] - y[0]), 32.f * (d[3] - y[1]));
+        rest[n][4 + i] = 0;
+      }
     }
     sb[n] = 127 + (int)fmaxf(base - c[n].m, -127.f);
   }
@@ -257,7 +246,10 @@ __device__ __forceinline__ void attend_tile(Columns<DC> (&c)[NT], const QueryTil
   constexpr int kOnes = 0x38383838;
   const i32x8 ones = {kOnes, kOnes, kOnes, kOnes, kOnes, kOnes, kOnes, kOnes};
 #pragma unroll
-  for (int n = 0; n < NT; ++n) c[n].l = mfma_e4m3(ones, pp[n], c[n].l, 127, sb[n]);
+  for (int n = 0; n < NT; ++n) {
+    c[n].l = mfma_e4m3(ones, pp[n], c[n].l, 127, sb[n]);
+    if constexpr (PIECES == 3) c[n].l = mfma_e4m3(ones, rest[n], c[n].l, 122, sb[n]);
+  }
   // Where part of the tile is hidden, what stands there may be anything, and 0 * NaN is NaN.
   bool nan = false;
   if (!whole) {
@@ -276,7 +268,10 @@ __device__ __forceinline__ void attend_tile(Columns<DC> (&c)[NT], const QueryTil
       const u32x4 v = kv.v(i);
       const i32x8 vv = pair8(v, v);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) c[n].o[i] = mfma_e4m3(vv, pp[n], c[n].o[i], sa, sb[n]);
+      for (int n = 0; n < NT; ++n) {
+        c[n].o[i] = mfma_e4m3(vv, pp[n], c[n].o[i], sa, sb[n]);
+        if constexpr (PIECES == 3) c[n].o[i] = mfma_e4m3(vv, rest[n], c[n].o[i], sa - 5, sb[n]);
+      }
     }
     return;
   }
@@ -303,6 +298,7 @@ __device__ __forceinline__ void attend_tile(Columns<DC> (&c)[NT], const QueryTil
         x[j] &= 0x38383838u;
       }
       c[n].o[i] = mfma_e4m3(pair8(v, v), pp[n], c[n].o[i], sa, sb[n]);
+      if constexpr (PIECES == 3) c[n].o[i] = mfma_e4m3(pair8(v, v), rest[n], c[n].o[i], sa - 5, sb[n]);
       const f32x4 sees = mfma_e4m3(pair8(x, zero), mine, f32x4{0.f, 0.f, 0.f, 0.f}, 127, 127);
 #pragma unroll
       for (int r = 0; r < 4; ++r) c[n].o[i][r] = sees[r] > 0.f ? __builtin_nanf("") : c[n].o[i][r];
