@@ -134,8 +134,6 @@ __device__ __forceinline__ void take_queries(QueryTile<DC, PIECES>& t, const Que
 template <int DC>
 struct KvRegs {
   u32x4 kr[4 * DC], vr[4 * DC];
-  __device__ __forceinline__ u32x4 k(int i) const { return kr[i]; }
-  __device__ __forceinline__ u32x4 v(int i) const { return vr[i]; }
   __device__ __forceinline__ void load(const uint8_t* kp, const uint8_t* vp, int lane) {
     const int at = (lane & 15) * 64 + (lane >> 4) * 16;
 #pragma unroll
@@ -158,6 +156,33 @@ __device__ __forceinline__ unsigned long long seen_keys(long first_key, long pos
   return m >> (4 * g);
 }
 
+// keys 16 i + 4 g + r of a tile that a query sees: bit 4 i + r
+__device__ __forceinline__ uint32_t seen_bits(long first_key, long pos, long length, int window, int keep, int g) {
+  const unsigned long long m = seen_keys(first_key, pos, length, window, keep, g);
+  return (uint32_t)(m & 0xf) | (uint32_t)(m >> 16 & 0xf) << 4 | (uint32_t)(m >> 32 & 0xf) << 8 | (uint32_t)(m >> 48 & 0xf) << 12;
+}
+
+// x *= f where it stands: a multiplication behind a branch would have the compiler copy every result on the other way round it. What it does not see into it does not
+// space from others either, so between_matrix() stands in front of such products, behind the instructions that make f, and behind them: 24 waits cover a matrix
+// instruction that writes x (16 passes: 19) and the exponential that gives f (1).
+__device__ __forceinline__ void between_matrix() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void times_here(f32x4& x, float f) {
+  float a = x[0], b = x[1], c = x[2], d = x[3];
+  asm volatile("v_mul_f32 %0, %4, %0\n\tv_mul_f32 %1, %4, %1\n\tv_mul_f32 %2, %4, %2\n\tv_mul_f32 %3, %4, %3" : "+v"(a), "+v"(b), "+v"(c), "+v"(d) : "v"(f));
+  x = f32x4{a, b, c, d};
+}
+
+// What a tile's score products are multiplied by. Not 0, which a query and keys of zeros would make it (2^-120 is a page's scale then): a hidden key's score is -inf. Nor more
+// than leaves the largest products finite.
+__device__ __forceinline__ float score_unit(float query, float keys) { return __builtin_amdgcn_fmed3f(query * keys, 0x1p-126f, 0x1p100f); }
+
+// Scores so far from zero that what a fused product keeps and a maximum has rounded away counts in an exponential: they are rounded first.
+__device__ __forceinline__ bool is_far(float most) { return fabsf(most) >= 0x1p22f && most > kNoMax; }
+
 // The running result of 16 columns: lane (column, g) has dimensions 16 i + 4 g + r.
 template <int DC>
 struct Columns {
@@ -172,91 +197,84 @@ struct Columns {
   }
 };
 
-// The tile's scores and values into the results of NT times 16 columns. pos: the lane's columns' positions (-1: no column); first_key: key 0 of the tile;
+// The tile's scores and values into the results of 16 columns. pos: the lane's column's position (-1: no column); first_key: key 0 of the tile;
 // whole: every column sees all 64 keys. `ks`, `vs`: the page's scales.
-template <int DC, int PIECES, int NT, typename KV>
-__device__ __forceinline__ void attend_tile(Columns<DC> (&c)[NT], const QueryTile<DC, PIECES> (&q)[NT], const KV& kv, float ks, float vs, bool whole, long first_key,
-                                            const long (&pos)[NT], long length, int window, int keep, int g) {
+template <int DC, int PIECES>
+__device__ __forceinline__ void attend_tile(Columns<DC>& c, const QueryTile<DC, PIECES>& q, const KvRegs<DC>& kv, float ks, float vs, bool whole, long first_key, long pos,
+                                            long length, int window, int keep, int g) {
   constexpr int M = (DC + 1) / 2;
   const u32x4 zero = {0, 0, 0, 0};
-  f32x4 s[NT][4];
+  f32x4 s[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      const i32x8 kk = pair8(kv.k(8 * m + i), 2 * m + 1 < DC ? kv.k(2 * m + 1 < DC ? 8 * m + 4 + i : 0) : zero);
+      const i32x8 kk = pair8(kv.kr[8 * m + i], 2 * m + 1 < DC ? kv.kr[2 * m + 1 < DC ? 8 * m + 4 + i : 0] : zero);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < PIECES; ++j) s[n][i] = mfma_e4m3(kk, q[n].piece[j][m], s[n][i], 127, 127 - 5 * j);
+      for (int j = 0; j < PIECES; ++j) s[i] = mfma_e4m3(kk, q.piece[j][m], s[i], 127, 127 - 5 * j);
     }
   }
-  i32x8 pp[NT], rest[NT];  // rest: fp16's third pieces, each 2^5 below what it adds to; the same values of the cache twice as in pp, the second time times zero
-  int sb[NT];
-  uint32_t seen[NT];  // keys 16 i + 4 g + r: bit 4 i + r
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    if (!whole) {
-      const unsigned long long m = seen_keys(first_key, pos[n], length, window, keep, g);
-      seen[n] = (uint32_t)(m & 0xf) | (uint32_t)(m >> 16 & 0xf) << 4 | (uint32_t)(m >> 32 & 0xf) << 8 | (uint32_t)(m >> 48 & 0xf) << 12;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[n][i][r] = seen[n] >> (4 * i + r) & 1u ? s[n][i][r] : -INFINITY;
-    }
-    const float unit = q[n].unit * ks;  // > 0
-    float most = s[n][0][0];
+  uint32_t seen = 0xffffu;
+  if (!whole) {
+    seen = seen_bits(first_key, pos, length, window, keep, g);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) most = fmaxf(most, s[n][i][r]);
-    most = rows_max(most) * unit;
-    const float mt = fmaxf(ceilf(fminf(most, 1e30f)), kNoMax);
-    if (__any(mt > c[n].m)) {
-      const float to = fmaxf(c[n].m, mt), f = __builtin_amdgcn_exp2f(c[n].m - to);
-      c[n].m = to;
-      c[n].l *= f;
-#pragma unroll
-      for (int i = 0; i < 4 * DC; ++i) c[n].o[i] *= f;
-    }
-    // probabilities of the tile, its largest in (2^7, 2^8]
-    const float base = fabsf(mt) < 1e8f ? mt - 8.f : mt;  // (beyond, the difference would be rounded)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float e[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[n][i][r], unit, -base));
-      const uint32_t hi = to_e4m3x4(e[0], e[1], e[2], e[3]);
-      const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true);
-      pp[n][i] = (int)hi;
-      const float d[4] = {e[0] - a[0], e[1] - a[1], e[2] - b[0], e[3] - b[1]};
-      const uint32_t lo = to_e4m3x4(d[0], d[1], d[2], d[3]);
-      pp[n][4 + i] = (int)lo;
-      if constexpr (PIECES == 3) {
-        const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, false), y = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, true);
-        rest[n][i] = (int)to_e4m3x4(32.f * (d[0] - x[0]), 32.f * (d[1] - x[1]), 32.f * (d[2] - y[0]), 32.f * (d[3] - y[1]));
-        rest[n][4 + i] = 0;
-      }
-    }
-    sb[n] = 127 + (int)fmaxf(base - c[n].m, -127.f);
+      for (int r = 0; r < 4; ++r) s[i][r] = seen >> (4 * i + r) & 1u ? s[i][r] : -INFINITY;
   }
-  const int sa = 127 + scale_exponent(vs);
+  float unit = score_unit(q.unit, ks);
+  float most = s[0][0];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) most = fmaxf(most, s[i][r]);
+  most = rows_max(most) * unit;
+  const float mt = fmaxf(ceilf(most), kNoMax);
+  if (__any(is_far(mt))) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) times_here(s[i], unit);
+    unit = 1.f;
+  }
+  if (__any(mt > c.m)) {
+    const float to = fmaxf(c.m, mt), f = __builtin_amdgcn_exp2f(c.m - to);
+    c.m = to;
+    c.l *= f;
+#pragma unroll
+    for (int i = 0; i < 4 * DC; ++i) c.o[i] *= f;
+  }
+  // probabilities of the tile, its largest in (2^7, 2^8]
+  const float base = fabsf(mt) < 0x1p24f ? mt - 8.f : mt;  // (beyond, the difference would be rounded)
+  i32x8 pp, rest;  // rest: fp16's third pieces, each 2^5 below what it adds to; the same values of the cache twice as in pp, the second time times zero
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float e[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], unit, -base));
+    const uint32_t hi = to_e4m3x4(e[0], e[1], e[2], e[3]);
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true);
+    pp[i] = (int)hi;
+    const float d[4] = {e[0] - a[0], e[1] - a[1], e[2] - b[0], e[3] - b[1]};
+    const uint32_t lo = to_e4m3x4(d[0], d[1], d[2], d[3]);
+    pp[4 + i] = (int)lo;
+    if constexpr (PIECES == 3) {
+      const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, false), y = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, true);
+      rest[i] = (int)to_e4m3x4(32.f * (d[0] - x[0]), 32.f * (d[1] - x[1]), 32.f * (d[2] - y[0]), 32.f * (d[3] - y[1]));
+      rest[4 + i] = 0;
+    }
+  }
+  const int sb = 127 + (int)fmaxf(base - c.m, -127.f), sa = 127 + scale_exponent(vs);
   constexpr int kOnes = 0x38383838;
   const i32x8 ones = {kOnes, kOnes, kOnes, kOnes, kOnes, kOnes, kOnes, kOnes};
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    c[n].l = mfma_e4m3(ones, pp[n], c[n].l, 127, sb[n]);
-    if constexpr (PIECES == 3) c[n].l = mfma_e4m3(ones, rest[n], c[n].l, 122, sb[n]);
-  }
+  c.l = mfma_e4m3(ones, pp, c.l, 127, sb);
+  if constexpr (PIECES == 3) c.l = mfma_e4m3(ones, rest, c.l, 122, sb);
   // Where part of the tile is hidden, what stands there may be anything, and 0 * NaN is NaN.
   bool nan = false;
   if (!whole) {
     uint32_t found = 0;
 #pragma unroll
     for (int i = 0; i < 4 * DC; ++i) {
-      const u32x4 v = kv.v(i);
+      const u32x4 v = kv.vr[i];
       found |= nan_bytes(v.x) | nan_bytes(v.y) | nan_bytes(v.z) | nan_bytes(v.w);
       __builtin_amdgcn_sched_barrier(0);  // (one chunk at a time here and below: kept apart, these rare steps cost the others no registers)
     }
@@ -265,44 +283,37 @@ __device__ __forceinline__ void attend_tile(Columns<DC> (&c)[NT], const QueryTil
   if (!nan) {
 #pragma unroll
     for (int i = 0; i < 4 * DC; ++i) {
-      const u32x4 v = kv.v(i);
-      const i32x8 vv = pair8(v, v);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        c[n].o[i] = mfma_e4m3(vv, pp[n], c[n].o[i], sa, sb[n]);
-        if constexpr (PIECES == 3) c[n].o[i] = mfma_e4m3(vv, rest[n], c[n].o[i], sa - 5, sb[n]);
-      }
+      const i32x8 vv = pair8(kv.vr[i], kv.vr[i]);
+      c.o[i] = mfma_e4m3(vv, pp, c.o[i], sa, sb);
+      if constexpr (PIECES == 3) c.o[i] = mfma_e4m3(vv, rest, c.o[i], sa - 5, sb);
     }
     return;
   }
   // A NaN code counts as zero, and a column that sees it gets a NaN.
+  i32x8 mine;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    i32x8 mine;
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t w = 0;
+    for (int r = 0; r < 4; ++r) w |= seen >> (4 * i + r) & 1u ? 0x38u << (8 * r) : 0u;
+    mine[i] = (int)w;
+    mine[4 + i] = 0;
+  }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) w |= seen[n] >> (4 * i + r) & 1u ? 0x38u << (8 * r) : 0u;
-      mine[i] = (int)w;
-      mine[4 + i] = 0;
+  for (int i = 0; i < 4 * DC; ++i) {
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 v = kv.vr[i], x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = nan_bytes(v[j]);
+      v[j] &= ~x[j];
+      x[j] &= 0x38383838u;
     }
+    c.o[i] = mfma_e4m3(pair8(v, v), pp, c.o[i], sa, sb);
+    if constexpr (PIECES == 3) c.o[i] = mfma_e4m3(pair8(v, v), rest, c.o[i], sa - 5, sb);
+    const f32x4 sees = mfma_e4m3(pair8(x, zero), mine, f32x4{0.f, 0.f, 0.f, 0.f}, 127, 127);
 #pragma unroll
-    for (int i = 0; i < 4 * DC; ++i) {
-      __builtin_amdgcn_sched_barrier(0);
-      u32x4 v = kv.v(i), x;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[j] = nan_bytes(v[j]);
-        v[j] &= ~x[j];
-        x[j] &= 0x38383838u;
-      }
-      c[n].o[i] = mfma_e4m3(pair8(v, v), pp[n], c[n].o[i], sa, sb[n]);
-      if constexpr (PIECES == 3) c[n].o[i] = mfma_e4m3(pair8(v, v), rest[n], c[n].o[i], sa - 5, sb[n]);
-      const f32x4 sees = mfma_e4m3(pair8(x, zero), mine, f32x4{0.f, 0.f, 0.f, 0.f}, 127, 127);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) c[n].o[i][r] = sees[r] > 0.f ? __builtin_nanf("") : c[n].o[i][r];
-    }
+    for (int r = 0; r < 4; ++r) c.o[i][r] = sees[r] > 0.f ? __builtin_nanf("") : c.o[i][r];
   }
   __builtin_amdgcn_sched_barrier(0);
 }
@@ -423,30 +434,30 @@ __global__ void __launch_bounds__(64 * W, DC == 4 ? W / 4 : 2) paged_columns_ker
     const int col = cb.first + (lane & 15);
     const bool there = col < cb.end;
     const int token = (unsigned)(there ? col : cb.end - 1) / (unsigned)p.group, head = h * p.group + (there ? col : cb.end - 1) - token * p.group;
-    const long pos[1] = {there ? sp.start + token : -1};
+    const long pos = there ? sp.start + token : -1;
     const QueryRow<DC> query = request_queries<DC>(p.q + (long)(sp.row0 + token) * p.q_tok + (long)head * p.q_head, g);
-    Columns<DC> c[1];
-    c[0].clear();
+    Columns<DC> c;
+    c.clear();
     auto page_of = [&](int i) { return i < end ? paged_page(p.t, b, range.at(i) >> per_page) : -1; };
     KvRegs<DC> t;
     int page = page_of(tile0 + wave);
     TilePlace at = tile_place(p, page, range.at(tile0 + wave), h);
     if (page >= 0) t.load(p.kp + at.at * (64 * D), p.vp + at.at * (64 * D), lane);
-    QueryTile<DC, PIECES> q[1];
-    take_queries<T, DC, PIECES>(q[0], query, there, p.scale, g);
+    QueryTile<DC, PIECES> q;
+    take_queries<T, DC, PIECES>(q, query, there, p.scale, g);
     for (int i = tile0 + wave; i < end; i += W) {
       const int page1 = page_of(i + W);
       if (page >= 0) {
         const long k0 = 64L * range.at(i);
-        attend_tile<DC, PIECES, 1>(c, q, t, at.ks, at.vs, sees_whole(p, k0, cb.pos0, cb.pos1, sp.length), k0, pos, sp.length, p.window, p.keep, g);
+        attend_tile<DC, PIECES>(c, q, t, at.ks, at.vs, sees_whole(p, k0, cb.pos0, cb.pos1, sp.length), k0, pos, sp.length, p.window, p.keep, g);
       }
       page = page1;
       at = tile_place(p, page, range.at(i + W), h);
       if (page >= 0) t.load(p.kp + at.at * (64 * D), p.vp + at.at * (64 * D), lane);
     }
 #pragma unroll
-    for (int i = 0; i < 4 * DC; ++i) *(f32x4*)&so[wave][lane & 15][16 * i + 4 * g] = c[0].o[i];
-    if (g == 0) { sm[wave][lane & 15] = c[0].m; sl[wave][lane & 15] = c[0].l[0]; }
+    for (int i = 0; i < 4 * DC; ++i) *(f32x4*)&so[wave][lane & 15][16 * i + 4 * g] = c.o[i];
+    if (g == 0) { sm[wave][lane & 15] = c.m; sl[wave][lane & 15] = c.l[0]; }
     __syncthreads();
     const int cc = threadIdx.x / (4 * W), in = threadIdx.x % (4 * W), my = cb.first + cc;  // 4 W threads per column
     if (my < cb.end) {
@@ -550,7 +561,7 @@ __global__ void __launch_bounds__(256) paged_join_units_kernel(const PagedAttnPa
 // the largest still has all its bits and what is 2^-31 of it some; bf16 has the exponents for anything.
 template <typename T> struct PromptType;
 template <> struct PromptType<BF16> {
-  static constexpr float kBias = 0.f, kRoom = 60.f;
+  static constexpr float kBias = 0.f, kRoom = 8.f;
   static constexpr uint32_t kOne = 0x3f80u;
   static __device__ __forceinline__ uint32_t codes(uint32_t w, float s, bool high) {
     return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true)) : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
@@ -563,20 +574,6 @@ template <> struct PromptType<F16> {
     return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true)) : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false));
   }
 };
-
-// x *= f where it stands: a multiplication behind a branch would have the compiler copy every result on the other way round it. What it does not see into it does not
-// space from others either, so between_matrix() stands in front of such products, behind the instructions that make f, and behind them: 24 waits cover a matrix
-// instruction that writes x (16 passes: 19) and the exponential that gives f (1).
-__device__ __forceinline__ void between_matrix() {
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-}
-__device__ __forceinline__ void times_here(f32x4& x, float f) {
-  float a = x[0], b = x[1], c = x[2], d = x[3];
-  asm volatile("v_mul_f32 %0, %4, %0\n\tv_mul_f32 %1, %4, %1\n\tv_mul_f32 %2, %4, %2\n\tv_mul_f32 %3, %4, %3" : "+v"(a), "+v"(b), "+v"(c), "+v"(d) : "v"(f));
-  x = f32x4{a, b, c, d};
-}
 
 template <int DC>
 struct PromptColumns {
@@ -614,27 +611,32 @@ __device__ __forceinline__ void prompt_scores(f32x4 (&s)[NT][4], const QueryTile
   }
 }
 
-// keys 16 i + 4 g + r of a tile that a query sees: bit 4 i + r
-__device__ __forceinline__ uint32_t seen_bits(long first_key, long pos, long length, int window, int keep, int g) {
-  const unsigned long long m = seen_keys(first_key, pos, length, window, keep, g);
-  return (uint32_t)(m & 0xf) | (uint32_t)(m >> 16 & 0xf) << 4 | (uint32_t)(m >> 32 & 0xf) << 8 | (uint32_t)(m >> 48 & 0xf) << 12;
-}
-
 // The reference of the probabilities moves where the tile's largest score (of this lane's keys) passes it by kRoom.
 template <typename T, int DC, int NT>
-__device__ __forceinline__ void prompt_move(PromptColumns<DC> (&c)[NT], const float (&most)[NT]) {
+__device__ __forceinline__ void prompt_move(PromptColumns<DC> (&c)[NT], const float (&most)[NT], f32x4 (&s)[NT][4], float (&unit)[NT]) {
   typedef PromptType<T> PT;
-  bool moves = false;
+  bool moves = false, far = false;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) moves |= most[n] > c[n].m + PT::kRoom;
+  for (int n = 0; n < NT; ++n) {
+    moves |= most[n] > c[n].m + PT::kRoom;
+    far |= is_far(most[n]);
+  }
+  if (__any(far)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) times_here(s[n][i], unit[n]);
+      unit[n] = 1.f;
+    }
+  }
   if (__any(moves)) {
     float f[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {  // (a column's four lanes move together)
-      const float mt = fmaxf(ceilf(fminf(rows_max(most[n]), 1e30f)), kNoMax), to = mt > c[n].m + PT::kRoom ? mt : c[n].m;
+      const float mt = fmaxf(ceilf(rows_max(most[n])), kNoMax), to = mt > c[n].m + PT::kRoom ? mt : c[n].m;
       f[n] = __builtin_amdgcn_exp2f(c[n].m - to);
       c[n].m = to;
-      c[n].to = fabsf(to) < 1e8f ? PT::kBias - to : -to;  // (beyond, the sum would be rounded)
+      c[n].to = fabsf(to) < 0x1p24f ? PT::kBias - to : -to;  // (beyond, the sum would be rounded)
     }
     between_matrix();
 #pragma unroll
@@ -720,11 +722,11 @@ __device__ __forceinline__ void prompt_nans(PromptColumns<DC> (&c)[NT], const ui
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// A workgroup of W waves takes W NT times 16 columns of one KV head (NT times 16 a wave) and `split_tiles` tiles, which its waves share through LDS: two tiles' room, the
+// A workgroup of four waves takes 64 NT columns of one KV head (16 NT a wave) and `split_tiles` tiles, which its waves share through LDS: two tiles' room, the
 // next one's keys on their way to LDS and its values to registers while the waves work on one, one barrier a tile.
-template <typename T, int DC, int PIECES, int NT, int W>
-__global__ void __launch_bounds__(64 * W, W / 4 * (DC == 4 ? 1 : 2)) paged_tiles_kernel(const PagedAttnParams p) {
-  constexpr int D = DC * 64, kCols = 16 * W * NT, kMine = (4 * DC + W - 1) / W;  // chunks of a tile that a wave fetches
+template <typename T, int DC, int PIECES, int NT>
+__global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const PagedAttnParams p) {
+  constexpr int D = DC * 64, kCols = 64 * NT;
   typedef PromptType<T> PT;
   __shared__ u32x4 keys[2][64 * D / 16], values[2][64 * D / 8];
   __shared__ int nan_tile[2];  // number of the tile + 1 where its values hold a NaN (looked for, and taken out, where not every column sees all of it)
@@ -766,16 +768,14 @@ __global__ void __launch_bounds__(64 * W, W / 4 * (DC == 4 ? 1 : 2)) paged_tiles
   const int lane_at = (lane & 15) * 64 + (lane >> 4) * 16;
   auto page_of = [&](int i) { return i < end ? __builtin_amdgcn_readfirstlane(paged_page(p.t, b, cb.range.at(i) >> per_page)) : -1; };
   auto fetch_keys = [&](const TilePlace& at, int slot) {
-    if (4 * DC < W && wave >= 4 * DC) return;
 #pragma unroll
-    for (int i = 0; i < kMine; ++i)
-      load_lds16((const uint16_t*)(p.kp + at.at * (64 * D) + (wave * kMine + i) * 1024 + lane_at), (uint16_t*)&keys[slot][(wave * kMine + i) * 64]);
+    for (int i = 0; i < DC; ++i)
+      load_lds16((const uint16_t*)(p.kp + at.at * (64 * D) + (wave * DC + i) * 1024 + lane_at), (uint16_t*)&keys[slot][(wave * DC + i) * 64]);
   };
-  u32x4 raw[kMine];
+  u32x4 raw[DC];
   auto fetch_values = [&](const TilePlace& at) {
-    if (4 * DC < W && wave >= 4 * DC) return;
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) raw[i] = ld16(p.vp + at.at * (64 * D) + (wave * kMine + i) * 1024 + lane_at);
+    for (int i = 0; i < DC; ++i) raw[i] = ld16(p.vp + at.at * (64 * D) + (wave * DC + i) * 1024 + lane_at);
   };
   // fp16 holds a page's values times 2^(7 - loudest) of the loudest page so far: all codes exactly, unless a page is 2^22 times quieter than another
   int loudest = -126;
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(64 * W, W / 4 * (DC == 4 ? 1 : 2)) paged_tiles
     if (!sees_whole(p, 64L * cb.range.at(tile_no), cb.pos0, cb.pos1, sp.length)) {
       uint32_t found = 0;
 #pragma unroll
-      for (int i = 0; i < kMine; ++i)
+      for (int i = 0; i < DC; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t n = nan_bytes(raw[i][j]);
@@ -807,13 +807,12 @@ __global__ void __launch_bounds__(64 * W, W / 4 * (DC == 4 ? 1 : 2)) paged_tiles
       }
       s = exp2i(e - loudest + 7 < -126 ? -126 : e - loudest + 7);
     }
-    if (4 * DC < W && wave >= 4 * DC) return;
 #pragma unroll
-    for (int i = 0; i < kMine; ++i)
+    for (int i = 0; i < DC; ++i)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint32_t a = raw[i][2 * half], d = raw[i][2 * half + 1];
-        values[slot][((wave * kMine + i) * 2 + half) * 64 + lane] = u32x4{PT::codes(a, s, false), PT::codes(a, s, true), PT::codes(d, s, false), PT::codes(d, s, true)};
+        values[slot][((wave * DC + i) * 2 + half) * 64 + lane] = u32x4{PT::codes(a, s, false), PT::codes(a, s, true), PT::codes(d, s, false), PT::codes(d, s, true)};
       }
   };
   // Tile i's probabilities and value products go with tile i + 1's scores: while the vector ALU takes exponentials the matrix cores have products that wait for nothing.
@@ -853,10 +852,10 @@ __global__ void __launch_bounds__(64 * W, W / 4 * (DC == 4 ? 1 : 2)) paged_tiles
     prompt_most<NT>(most, s);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      unit[n] = q[n].unit * at.ks;
+      unit[n] = score_unit(q[n].unit, at.ks);
       most[n] *= unit[n];
     }
-    prompt_move<T, DC, NT>(c, most);
+    prompt_move<T, DC, NT>(c, most, s, unit);
   }
   int i = begin;
   auto step = [&](auto whole) {
@@ -890,11 +889,11 @@ __global__ void __launch_bounds__(64 * W, W / 4 * (DC == 4 ? 1 : 2)) paged_tiles
     prompt_most<NT>(most, s);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      unit[n] = q[n].unit * at1.ks;
+      unit[n] = score_unit(q[n].unit, at1.ks);
       most[n] *= unit[n];
     }
     if (page1 >= 0) put_values(at1, slot ^ 1, i + 1);
-    if (kWhole || i + 1 < end) prompt_move<T, DC, NT>(c, most);
+    if (kWhole || i + 1 < end) prompt_move<T, DC, NT>(c, most, s, unit);
     at1 = at2;
     page = page1;
     page1 = page2;
@@ -969,6 +968,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
 struct PagedPlan { int block_cols, col_tiles, split_tiles, splits, waves, workgroups; size_t scratch; };
 static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_length, int window, int keep, int n_q_heads, int n_kv_heads, int head_dim) {
   PagedPlan r = {};
+  if (max_tokens > n_rows) max_tokens = n_rows;
   const long group = n_q_heads / n_kv_heads;
   const bool prompt = max_tokens * group > 64;
   r.block_cols = prompt ? (head_dim == 256 ? 64 : 128) : 16;  // (256 dimensions: results of 32 columns a wave do not fit its registers)
@@ -1058,7 +1058,7 @@ extern "C" int mui_paged_attention(mui_stream_t stream, int dtype, const void* q
 #define MUI_PAGED_GO(TT, DC, PIECES)                                                                                                       \
   do {                                                                                                                                     \
     if (prompt) {                                                                                                                          \
-      hipLaunchKernelGGL((paged_tiles_kernel<TT, DC, PIECES, DC == 4 ? 1 : 2, 4>), dim3((unsigned)blocks, plan.splits), dim3(256), 0, s, p); \
+      hipLaunchKernelGGL((paged_tiles_kernel<TT, DC, PIECES, DC == 4 ? 1 : 2>), dim3((unsigned)blocks, plan.splits), dim3(256), 0, s, p); \
       if (p.part) hipLaunchKernelGGL((paged_join_kernel<TT, DC>), join, dim3(256), 0, s, p);                                               \
     } else {                                                                                                                               \
       if constexpr (DC < 4) {                                                                                                              \

@@ -1373,6 +1373,8 @@ def mui_sample_filtered(logits: torch.Tensor, random_numbers: torch.Tensor, temp
         raise RuntimeError("logits have no vocabulary")
     l2 = logits if logits.dim() == 2 else logits.reshape(-1, v)
     rows, f32 = l2.shape[0], torch.float32
+    if rows > 1 and l2.stride(0) < v:
+        l2 = l2.contiguous()
     us, _ = _per_row(random_numbers, "random_numbers", rows, f32, at, None)
     if us is None:
         raise RuntimeError(f"random_numbers must be a contiguous {f32} tensor of {rows}")
@@ -1382,6 +1384,7 @@ def mui_sample_filtered(logits: torch.Tensor, random_numbers: torch.Tensor, temp
     ms, m = _per_row(min_p, "min_p", rows, f32, at, 0.0)
     if not t >= 0 or not p >= 0 or not 0 <= m <= 1 or k < 0:
         raise ValueError("temperature, top_k and top_p must not be negative, min_p must lie in 0 .. 1")
+    k = min(k, v)
     token, probability = l2.new_empty(rows, dtype=torch.int64), l2.new_empty(rows, dtype=f32)
     if rows == 0:
         return token, probability

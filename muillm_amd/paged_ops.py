@@ -119,16 +119,31 @@ def _dtype(x: torch.Tensor) -> int:
     return code
 
 
+def _most_tokens(max_tokens: Optional[int], offsets: Optional[torch.Tensor], n_rows: int) -> int:
+    if max_tokens is None:
+        return 1 if offsets is None else n_rows
+    if max_tokens < 1:
+        raise RuntimeError("max_tokens must be positive")
+    return min(max_tokens, n_rows)
+
+
 @functools.lru_cache(maxsize=1024)
 def _scratch_bytes(*sizes: int) -> int:
     return _lib.load().mui_paged_attention_scratch_bytes(*sizes)
 
 
-def _output(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
+def _output(out: Optional[torch.Tensor], q: torch.Tensor, in_place: bool) -> torch.Tensor:
     if out is None:
         return q.new_empty(q.shape)
     if out.dtype is not q.dtype or out.shape != q.shape or not out.is_contiguous() or out.get_device() != q.get_device():
         raise RuntimeError("out must be a contiguous tensor of q's shape and type")
+    if in_place and out.data_ptr() == q.data_ptr() and q.is_contiguous():
+        return out
+    rows, heads, dim = q.shape
+    begin, size = q.data_ptr(), q.element_size()
+    end = begin + size * ((rows - 1) * q.stride(0) + (heads - 1) * q.stride(1) + dim)
+    if out.numel() and begin < out.data_ptr() + size * out.numel() and out.data_ptr() < end:
+        raise RuntimeError("out must not lie over q" + (", unless it is q" if in_place else ""))
     return out
 
 
@@ -144,7 +159,8 @@ def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, kv
 
     A page's scale is the smallest power of two with which its largest value fits 448, and does not fall while earlier tokens stand there; where it
     rises their codes follow. Infinities and NaN become NaN. A page that is appended to belongs to one request. Tokens without a place (a table entry that is no
-    page, a length beyond the table) are not written. max_tokens: at least the most new tokens of a request (default: 1 without offsets, else all rows)."""
+    page, a length beyond the table) are not written. max_tokens: at least the most new tokens of a request (default: 1 without offsets, else all rows): 1 takes
+    the kernel for single tokens, others' tokens behind the first are then not appended. out may be q itself."""
     n_rows = k.shape[0]
     n, width, step = _places(kv, table, lengths, offsets, n_rows)
     code, dtype = _dtype(k), k.dtype
@@ -154,7 +170,7 @@ def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, kv
     qp = op = fp = None
     if q is not None:
         heads, qt, qh = _rows(q, "q", kv, None, dtype, n_rows)
-        out = _output(out, q)
+        out = _output(out, q, True)
         qp, op = q.data_ptr(), out.data_ptr()
     rot = 0
     if inv_freq is not None:
@@ -167,8 +183,7 @@ def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, kv
         raise RuntimeError(f"positions must be a contiguous int64 tensor [{n_rows}] on the cache's device")
     if n_rows == 0:
         return out if q is not None else None
-    if max_tokens is None:
-        max_tokens = 1 if offsets is None else n_rows
+    max_tokens = _most_tokens(max_tokens, offsets, n_rows)
     check(_call(kv.index, _lib.load().mui_paged_append, code, qp, qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, kv.k.data_ptr(), kv.v.data_ptr(),
                 kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.n_pages, kv.page, table.data_ptr(), step, width, lengths.data_ptr(),
                 None if offsets is None else offsets.data_ptr(), None if positions is None else positions.data_ptr(), fp, rot, 1 if interleaved else 0, rope_scale, op,
@@ -183,7 +198,8 @@ def paged_attention(q: torch.Tensor, kv: PagedKV, table: torch.Tensor, lengths: 
     new tokens already. scale > 0: of the scores (default dim ** -0.5). window > 0: a token sees the last `window` ones, itself among them, and the first
     keep_first of its request. A token that sees nothing gives zeros; keys on a table entry that is no page do not count.
 
-    max_tokens: as in paged_append; max_length: at least the largest of lengths (default: what a row of the table can hold). Both only size the launch."""
+    max_tokens: as in paged_append; max_length: at least the largest of lengths (default: what a row of the table can hold). Both size the launch: tokens and keys
+    beyond what they say may be left out."""
     n_rows = q.shape[0]
     n, width, step = _places(kv, table, lengths, offsets, n_rows)
     code = _dtype(q)
@@ -196,11 +212,10 @@ def paged_attention(q: torch.Tensor, kv: PagedKV, table: torch.Tensor, lengths: 
         scale = kv.dim ** -0.5
     elif not scale > 0:
         raise RuntimeError("scale must be positive")
-    out = _output(out, q)
+    out = _output(out, q, False)
     if n_rows == 0:
         return out
-    if max_tokens is None:
-        max_tokens = 1 if offsets is None else n_rows
+    max_tokens, window, keep_first = _most_tokens(max_tokens, offsets, n_rows), min(window, 0x7fffffff), min(keep_first, 0x7fffffff)
     most = min(width * kv.page, 0x7fffffff)
     max_length = most if max_length is None else max(1, min(max_length, most))
     nbytes = _scratch_bytes(n_rows, n, max_tokens, max_length, window, keep_first, heads, kv.kv_heads, kv.dim)

@@ -111,3 +111,11 @@ def test_tensors_of_the_cpu_are_refused():
         paged_ops.paged_attention(x, kv, table, lengths)
     with pytest.raises(RuntimeError, match="CUDA"):
         muillm_ext.mui_sample_filtered(torch.zeros((1, 10), dtype=torch.float16), torch.zeros(1))
+
+
+@pytest.mark.parametrize("dim,heads", [(64, 8), (128, 8), (128, 4), (256, 2)])
+def test_a_bound_above_the_rows_asks_for_no_more(dim, heads):
+    lib = _lib.load()
+    for rows in (1, 7, 40, 200):
+        one = lib.mui_paged_attention_scratch_bytes(rows, 4, rows, 5000, 0, 0, heads, 2, dim)
+        assert one == lib.mui_paged_attention_scratch_bytes(rows, 4, 0x7fffffff, 5000, 0, 0, heads, 2, dim) < 1 << 30
