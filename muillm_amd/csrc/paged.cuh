@@ -58,11 +58,10 @@ __device__ __forceinline__ long uniform(long x) {
 }
 __device__ __forceinline__ PagedSpan uniform(PagedSpan s) { return {uniform(s.row0), uniform(s.count), uniform(s.start), uniform(s.length)}; }
 
-// the page of slot `slot` of request b's table, or -1 where that is none
-__device__ __forceinline__ int paged_page(const PagedTable& p, int b, int slot) {
-  const int page = slot < p.pages ? p.table[(long)b * p.stride + slot] : -1;
-  return page >= 0 && page < p.n_pages ? page : -1;
-}
+// the page of slot `slot` of request b's table, or -1 where that is none; in two steps, for those who have other work while the entry comes
+__device__ __forceinline__ int paged_entry(const PagedTable& p, int b, int slot) { return slot < p.pages ? p.table[(long)b * p.stride + slot] : -1; }
+__device__ __forceinline__ int page_of_entry(const PagedTable& p, int entry) { return entry >= 0 && entry < p.n_pages ? entry : -1; }
+__device__ __forceinline__ int paged_page(const PagedTable& p, int b, int slot) { return page_of_entry(p, paged_entry(p, b, slot)); }
 
 // 2^e, -126 <= e <= 127
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }

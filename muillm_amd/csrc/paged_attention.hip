@@ -722,6 +722,62 @@ __device__ __forceinline__ void prompt_nans(PromptColumns<DC> (&c)[NT], const ui
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// The requests' blocks of PER columns, those first whose last column stands furthest behind (it sees most keys; of 64 requests at a time): the n-th one's request, number and
+// the request's rows. Every wave looks for itself, a request a lane. A block's place is counted in blocks too: the request's tokens times heads, and down from there.
+template <int PER>
+__device__ __forceinline__ bool nth_block(const PagedAttnParams& p, int n, int& b, int& block, PagedSpan& sp) {
+  const int lane = threadIdx.x & 63;
+  auto of = [](int x, int l) { return __builtin_amdgcn_readlane(x, l); };
+  auto of_long = [&](long x, int l) { return (long)((unsigned long long)(uint32_t)of((int)(x >> 32), l) << 32 | (uint32_t)of((int)(x & 0xffffffffL), l)); };
+  for (int r0 = 0; r0 < p.t.n_requests; r0 += kWave) {
+    PagedSpan s = {};
+    int blocks = 0, top = 0;
+    if (r0 + lane < p.t.n_requests) {
+      s = paged_span(p.t, r0 + lane);
+      blocks = (s.count * p.group + PER - 1) / PER;
+      const long last = s.length * p.group / PER;
+      top = last < (1 << 30) ? (int)last : 1 << 30;
+    }
+    const int here = p.t.n_requests - r0 < kWave ? p.t.n_requests - r0 : kWave;
+    int total = 0, high = 0, low = 1 << 30;  // the places there are
+    for (int r = 0; r < here; ++r) {
+      const int t = of(top, r), m = of(blocks, r);
+      total += m;
+      high = t > high ? t : high;
+      low = m && t - m + 1 < low ? t - m + 1 : low;
+    }
+    if (n >= total) {
+      n -= total;
+      continue;
+    }
+    // the last place from which on there are more than n blocks, a place a lane
+    int step, front = 0;  // front: blocks behind it
+    do {
+      step = (high - low) / kWave + 1;
+      const int place = low + lane * step;
+      int from = 0, behind = 0;
+      for (int r = 0; r < here; ++r) {
+        const int mine = of(top, r) - place + 1, m = of(blocks, r);
+        from += mine < 0 ? 0 : mine < m ? mine : m;
+        behind += mine < 1 ? 0 : mine - 1 < m ? mine - 1 : m;
+      }
+      const int last = 63 - __clzll((long long)__ballot(from > n));
+      front = of(behind, last);
+      low += last * step;
+      high = low + step - 1;
+    } while (step > 1);
+    n -= front;
+    const int down = top - low;
+    const unsigned long long at = __ballot(down >= 0 && down < blocks);
+    const int l = __ffsll((long long)__ballot((at >> lane & 1ull) && __popcll(at & ((1ull << lane) - 1ull)) == n)) - 1;
+    b = r0 + l;
+    block = of(blocks - 1 - down, l);
+    sp = {of(s.row0, l), of(s.count, l), of_long(s.start, l), of_long(s.length, l)};
+    return true;
+  }
+  return false;
+}
+
 // A workgroup of four waves takes 64 NT columns of one KV head (16 NT a wave) and `split_tiles` tiles, which its waves share through LDS: two tiles' room, the
 // next one's keys on their way to LDS and its values to registers while the waves work on one, one barrier a tile.
 template <typename T, int DC, int PIECES, int NT>
@@ -731,12 +787,10 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
   __shared__ u32x4 keys[2][64 * D / 16], values[2][64 * D / 8];
   __shared__ int nan_tile[2];  // number of the tile + 1 where its values hold a NaN (looked for, and taken out, where not every column sees all of it)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Neighbouring blocks go to different XCDs: those of one request and KV head, which read the same keys, lie a multiple of n_requests * kv_heads apart. The
-  // last columns see most: they come first.
-  const unsigned units = p.t.n_requests * p.kv_heads;
-  const int b = blockIdx.x % units / p.kv_heads, h = blockIdx.x % units % p.kv_heads, ct = p.col_tiles - 1 - blockIdx.x / units;
-  const PagedSpan sp = uniform(paged_span(p.t, b));
-  if (kCols * ct >= sp.count * p.group) return;
+  const int h = blockIdx.x % p.kv_heads;  // (neighbours go to different XCDs: of eight heads each XCD has one, whose keys stay in its L2)
+  int b, ct;
+  PagedSpan sp;
+  if (!nth_block<kCols>(p, blockIdx.x / p.kv_heads, b, ct, sp)) return;
   const ColumnBlock cb = column_block(p, sp, ct, kCols);
   const int n_tiles = cb.range.count();
   const int begin = blockIdx.y * p.split_tiles;
@@ -766,7 +820,9 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
   }
   const int per_page = p.t.page_shift - 6;
   const int lane_at = (lane & 15) * 64 + (lane >> 4) * 16;
-  auto page_of = [&](int i) { return i < end ? __builtin_amdgcn_readfirstlane(paged_page(p.t, b, cb.range.at(i) >> per_page)) : -1; };
+  // a tile's page is loaded a tile before it is looked at: what follows would wait for it
+  auto entry_of = [&](int i) { return i < end ? paged_entry(p.t, b, cb.range.at(i) >> per_page) : -1; };
+  auto page_of = [&](int entry) { return uniform(page_of_entry(p.t, entry)); };
   auto fetch_keys = [&](const TilePlace& at, int slot) {
 #pragma unroll
     for (int i = 0; i < DC; ++i)
@@ -777,10 +833,18 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
 #pragma unroll
     for (int i = 0; i < DC; ++i) raw[i] = ld16(p.vp + at.at * (64 * D) + (wave * DC + i) * 1024 + lane_at);
   };
+  // tiles that all columns see: in front of the first's end and, with a window, in it for the last, or among the first keys
+  const long whole_end = cb.pos0 + 1 < sp.length ? (cb.pos0 + 1) >> 6 : sp.length >> 6;
+  const int seen_end = whole_end < 0 ? 0 : (int)whole_end, seen_kept = p.keep >> 6;
+  const int seen_from = p.window > 0 ? (int)((cb.pos1 - p.window) >> 6) + 1 : 0;
+  auto all_seen = [&](int tile_no) {
+    const int t = cb.range.at(tile_no);
+    return t < seen_end && (t >= seen_from || t < seen_kept);
+  };
   // fp16 holds a page's values times 2^(7 - loudest) of the loudest page so far: all codes exactly, unless a page is 2^22 times quieter than another
   int loudest = -126;
-  auto put_values = [&](const TilePlace& at, int slot, int tile_no) {
-    if (!sees_whole(p, 64L * cb.range.at(tile_no), cb.pos0, cb.pos1, sp.length)) {
+  auto put_values = [&](const TilePlace& at, int slot, int tile_no, auto whole) {
+    if (!decltype(whole)::value && !all_seen(tile_no)) {
       uint32_t found = 0;
 #pragma unroll
       for (int i = 0; i < DC; ++i)
@@ -817,7 +881,7 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
   };
   // Tile i's probabilities and value products go with tile i + 1's scores: while the vector ALU takes exponentials the matrix cores have products that wait for nothing.
   // A step begins with tile i's scores in registers, its values in LDS or about to be, tile i + 1's keys on their way to LDS.
-  int page = page_of(begin), page1 = page_of(begin + 1), page2 = page_of(begin + 2);
+  int page = page_of(entry_of(begin)), page1 = page_of(entry_of(begin + 1)), entry2 = entry_of(begin + 2);
   TilePlace at = tile_place(p, page, cb.range.at(begin), h), at1 = tile_place(p, page1, cb.range.at(begin + 1), h);
   f32x4 s[NT][4];
   float most[NT], unit[NT];
@@ -825,7 +889,7 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
   if (page >= 0) {
     fetch_keys(at, 0);
     fetch_values(at);
-    put_values(at, 0, begin);
+    put_values(at, 0, begin, std::false_type());
   }
   wait_loads<0>();
   __syncthreads();
@@ -863,10 +927,12 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
     const int slot = (i - begin) & 1;
     wait_loads<0>();
     __syncthreads();  // tile i's values and tile i + 1's keys are there, for all; the other rooms' readers are done
-    const int page3 = page_of(i + 3);
+    asm volatile("" : "+v"(entry2));  // (not looked at earlier: it would be waited for)
+    const int page2 = page_of(entry2);
+    entry2 = entry_of(i + 3);
     const TilePlace at2 = tile_place(p, page2, cb.range.at(i + 2), h);
     if (page2 >= 0) fetch_keys(at2, slot);
-    if (page1 >= 0) fetch_values(at1);
+    if (kWhole || page1 >= 0) fetch_values(at1);
     u32x4 pp[NT][2];
     const PromptTile here = {nullptr, &values[slot][lane]}, ahead = {&keys[slot ^ 1][lane], nullptr};
     prompt_exp<T, DC, NT>(pp, s, c, unit);
@@ -892,19 +958,15 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
       unit[n] = score_unit(q[n].unit, at1.ks);
       most[n] *= unit[n];
     }
-    if (page1 >= 0) put_values(at1, slot ^ 1, i + 1);
+    if (kWhole || page1 >= 0) put_values(at1, slot ^ 1, i + 1, whole);
     if (kWhole || i + 1 < end) prompt_move<T, DC, NT>(c, most, s, unit);
     at1 = at2;
     page = page1;
     page1 = page2;
-    page2 = page3;
     ++i;
   };
   // (a loop for tiles that all columns see and one for others: with both in one the compiler copied the results between their registers at every tile)
-  auto whole_now = [&]() {
-    return i + 1 < end && page >= 0 && page1 >= 0 && sees_whole(p, 64L * cb.range.at(i), cb.pos0, cb.pos1, sp.length) &&
-           sees_whole(p, 64L * cb.range.at(i + 1), cb.pos0, cb.pos1, sp.length);
-  };
+  auto whole_now = [&]() { return i + 1 < end && page >= 0 && page1 >= 0 && all_seen(i) && all_seen(i + 1); };
   while (i < end) {
     while (whole_now()) step(std::true_type());
     while (i < end && !whole_now()) step(std::false_type());
@@ -965,7 +1027,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   for (int j = 0; j < DC; ++j) p.out[item * D + 64 * j + lane] = T::pack(o[j] * inv);
 }
 
-struct PagedPlan { int block_cols, col_tiles, split_tiles, splits, waves, workgroups; size_t scratch; };
+struct PagedPlan { int block_cols, col_tiles, split_tiles, splits, waves, workgroups; long blocks; size_t scratch; };
 static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_length, int window, int keep, int n_q_heads, int n_kv_heads, int head_dim) {
   PagedPlan r = {};
   if (max_tokens > n_rows) max_tokens = n_rows;
@@ -979,7 +1041,10 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
     tiles = tiles < seen ? tiles : seen;
   }
   if (tiles < 1) tiles = 1;
-  const long units = (long)n_requests * n_kv_heads * r.col_tiles;
+  // (of prompts: no more than the rows fill, and one of each request that is not full)
+  const long filled = ((long)n_rows * group + r.block_cols - 1) / r.block_cols + n_requests;
+  r.blocks = n_kv_heads * (prompt && filled < (long)n_requests * r.col_tiles ? filled : (long)n_requests * r.col_tiles);
+  const long units = r.blocks;
   r.splits = 1;
   r.split_tiles = (int)tiles;
   if (prompt) {
@@ -1036,7 +1101,7 @@ extern "C" int mui_paged_attention(mui_stream_t stream, int dtype, const void* q
   if (plan.scratch && (!scratch || scratch_bytes < plan.scratch)) return MUI_ERR_INVALID_ARG;
   if ((long)n_rows * n_q_heads > 0x7fffffffL - 256) return MUI_ERR_UNSUPPORTED;
   const bool prompt = plan.block_cols > 16;
-  const long blocks = (long)plan.col_tiles * n_kv_heads * n_requests;
+  const long blocks = plan.blocks;
   if (blocks > 0x7fffffffL || plan.splits > 65535 || n_requests > 65535) return MUI_ERR_UNSUPPORTED;
   PagedAttnParams p = {};
   p.q = (const uint16_t*)q; p.q_tok = q_token_stride; p.q_head = q_head_stride;

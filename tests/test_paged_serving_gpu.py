@@ -369,3 +369,16 @@ def test_sampling_refusals_and_rows_that_share():
     assert token.tolist() == [pick(logits[0], float(x), 1.0, 0, 1.0, 0.0)[0] for x in u]
     turned = dev.t().contiguous().t()
     assert torch.equal(muillm_ext.mui_sample_filtered(turned, number)[0], muillm_ext.mui_sample_filtered(dev, number)[0])
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(F16, 128, 64), (BF16, 64, 128), (BF16, 256, 64)])
+def test_prompts_of_many_requests(dtype, dim, page):
+    """More than one wave's lanes of requests, some without tokens, some behind cached ones: every block is found once."""
+    g = torch.Generator().manual_seed(3)
+    new = torch.randint(0, 12, (150,), generator=g).tolist()
+    new[7], new[63], new[64], new[149] = 90, 70, 0, 65
+    lengths = [n + int(torch.randint(0, 50, (1,), generator=g)) for n in new]
+    lengths[10] += 700
+    run_attention(dtype, dim, page, lengths, new, 7, 1)
+    run_attention(dtype, dim, page, lengths, new, 8, 2, max_tokens=90)
+    run_attention(dtype, dim, page, lengths[:3] + [2000], [0, 0, 1, 300], 8, 1)
