@@ -833,38 +833,81 @@ int mui_channel_delta(mui_stream_t stream, int dtype, const mui_channel_delta_t*
  * largest length) size the launch; rows and keys beyond what they say may be left out.
  * ---------------------------------------------------------------------------------- */
 
-/* Rotates and appends. q [n_rows, n_q_heads, head_dim] (may be NULL), k, v [n_rows, n_kv_heads, head_dim] with strides in elements (multiples of 8); q_out dense.
+/* The calls' arguments come in structs, whose unused pointers are NULL; out of them nothing is kept.
+ *
+ * Rotates and appends. q [n_rows, n_q_heads, head_dim] (may be NULL), k, v [n_rows, n_kv_heads, head_dim] with strides in elements (multiples of 8); q_out dense (may be q).
  * The first rot_dim (a multiple of 16) dimensions of q and k turn by the angle position * inv_freq[i] (double [rot_dim / 2]; its whole turns dropped in double precision):
  * pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) if interleaved; cosine and sine times rope_scale. positions: int64 [n_rows], or NULL: a token's place in its request.
  * q_out is rounded once. Per page and head, over the tokens appended: scale = 2^e, e the smallest integer >= -120 with max |x| <= 448 * 2^e (infinities and NaN left
  * out), at least the scale that stands there if the page holds earlier tokens, whose codes are then multiplied by the quotient and rounded again; code = x / scale,
- * nearest even; infinities and NaN give NaN codes. A page that is appended to must belong to one request. Rows behind the last request are left as they are. */
-int mui_paged_append(mui_stream_t stream, int dtype, const void* q, long q_token_stride, long q_head_stride, const void* k, long k_token_stride,
-                     long k_head_stride, const void* v, long v_token_stride, long v_head_stride, void* k_pages, void* v_pages, float* k_scale,
-                     float* v_scale, int n_pages, int page_tokens, const int32_t* table, long table_stride, int table_pages, const int64_t* lengths,
-                     const int64_t* offsets, const int64_t* positions, const double* inv_freq, int rot_dim, int interleaved, float rope_scale,
-                     void* q_out, int n_rows, int n_requests, int max_tokens, int n_q_heads, int n_kv_heads, int head_dim);
+ * nearest even; infinities and NaN give NaN codes. A page that is appended to must belong to one request. Rows behind the last request are left as they are.
+ * max_tokens 1: only the first new token of a request is appended; any other number: all of them. */
+typedef struct mui_paged_append_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* k_pages;
+  void* v_pages;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* table;
+  const int64_t* lengths;
+  const int64_t* offsets;
+  const int64_t* positions;
+  const double* inv_freq;
+  void* q_out;
+  long q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, table_stride;
+  int dtype, n_pages, page_tokens, table_pages, n_rows, n_requests, max_tokens, n_q_heads, n_kv_heads, head_dim, rot_dim, interleaved;
+  float rope_scale;
+} mui_paged_append_args_t;
+int mui_paged_append(mui_stream_t stream, const mui_paged_append_args_t* args);
 
 /* Causal attention of q [n_rows, n_q_heads, head_dim] over the cache, which holds the new tokens already: out (dense) = softmax(scale * q . k) v over the keys at positions
  * s <= p, p that of the token, and s > p - window or s < keep_first if window > 0. n_q_heads a multiple of n_kv_heads, scale > 0. A token without a key gives
- * zeros. Keys that a token does not see do not touch it, whatever their codes are. scratch: mui_paged_attention_scratch_bytes() bytes, 16-byte aligned (NULL if 0). */
+ * zeros. Keys that a token does not see do not touch it, whatever their codes are. out must not lie over q. scratch: mui_paged_attention_scratch_bytes() bytes for
+ * max_length cut to table_pages * page_tokens, 16-byte aligned (NULL if 0). */
+typedef struct mui_paged_attention_args {
+  const void* q;
+  const void* k_pages;
+  const void* v_pages;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* table;
+  const int64_t* lengths;
+  const int64_t* offsets;
+  void* scratch;
+  void* out;
+  size_t scratch_bytes;
+  long q_token_stride, q_head_stride, table_stride;
+  int dtype, n_pages, page_tokens, table_pages, n_rows, n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads, head_dim;
+  float scale;
+} mui_paged_attention_args_t;
 size_t mui_paged_attention_scratch_bytes(int n_rows, int n_requests, int max_tokens, int max_length, int window, int keep_first, int n_q_heads, int n_kv_heads,
                                          int head_dim);
-int mui_paged_attention(mui_stream_t stream, int dtype, const void* q, long q_token_stride, long q_head_stride, const void* k_pages,
-                        const void* v_pages, const float* k_scale, const float* v_scale, int n_pages, int page_tokens, const int32_t* table,
-                        long table_stride, int table_pages, const int64_t* lengths, const int64_t* offsets, float scale, int window, int keep_first,
-                        int max_tokens, int max_length, void* scratch, size_t scratch_bytes, void* out, int n_rows, int n_requests, int n_q_heads,
-                        int n_kv_heads, int head_dim);
+int mui_paged_attention(mui_stream_t stream, const mui_paged_attention_args_t* args);
 
 /* Per row of 16-bit logits [rows, vocab]: a token from random_numbers[row], uniform in [0, 1). w_i = exp((l_i - max l) / temperature) in double precision; tokens in order of
  * falling logits, equal ones by rising index. Kept are the first top_k (<= 0: all); of those the ones in front of which less than top_p (>= 1: all) times the
  * top_k's weight lies; of those the ones with w >= min_p; the first one always. out_token = the first whose cumulative weight exceeds random_numbers[row] times
  * the kept weight, out_probability (may be NULL) its share of it. temperature <= 0: the largest logit. NaN and -inf are never drawn; a row of nothing else gives token 0
- * and probability 0. Each setting is an array of one per row or, where that is NULL, the number behind it. workspace: 16-byte aligned, what it holds does not matter. */
+ * and probability 0. Each setting is an array of one per row or, where that is NULL, the number of that name. workspace: 16-byte aligned, what it holds does not matter. */
+typedef struct mui_sample_filtered_args {
+  const void* logits;
+  const float* random_numbers;
+  const float* temperatures;
+  const int32_t* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+  int64_t* out_token;
+  float* out_probability;
+  void* workspace;
+  size_t workspace_bytes;
+  long row_stride;
+  int dtype, rows, vocab, top_k;
+  float temperature, top_p, min_p;
+} mui_sample_filtered_args_t;
 size_t mui_sample_filtered_workspace_bytes(int rows, int vocab);
-int mui_sample_filtered(mui_stream_t stream, int dtype, const void* logits, long row_stride, int rows, int vocab, const float* random_numbers,
-                        const float* temperatures, float temperature, const int32_t* top_ks, int top_k, const float* top_ps, float top_p,
-                        const float* min_ps, float min_p, int64_t* out_token, float* out_probability, void* workspace, size_t workspace_bytes);
+int mui_sample_filtered(mui_stream_t stream, const mui_sample_filtered_args_t* args);
 
 #ifdef __cplusplus
 }

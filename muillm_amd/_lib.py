@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import re
 from ctypes import c_char_p, c_float, c_int, c_long, c_void_p
 from typing import Dict, List, Optional
@@ -157,12 +158,11 @@ _SIGNATURES = {
     "mui_channel_delta_max_tokens": (c_int, [c_int, c_int]),
     "mui_channel_delta_workspace_bytes": (ctypes.c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "mui_channel_delta": (c_int, [_P, c_int, _P, _P, c_long, _P, _P, _P, _P, _P, _P, c_int, c_int]),
-    "mui_paged_append": (c_int, [_P, c_int] + [_P, c_long, c_long] * 3 + [_P, _P, _P, _P, c_int, c_int, _P, c_long, c_int, _P, _P, _P, _P, c_int, c_int, c_float, _P] + [c_int] * 6),
+    "mui_paged_append": (c_int, [_P, c_char_p]),  # packed by the Struct below
     "mui_paged_attention_scratch_bytes": (ctypes.c_size_t, [c_int] * 9),
-    "mui_paged_attention": (c_int, [_P, c_int, _P, c_long, c_long, _P, _P, _P, _P, c_int, c_int, _P, c_long, c_int, _P, _P, c_float, c_int, c_int, c_int, c_int, _P,
-                                    ctypes.c_size_t, _P] + [c_int] * 5),
+    "mui_paged_attention": (c_int, [_P, c_char_p]),  # packed by the Struct below
     "mui_sample_filtered_workspace_bytes": (ctypes.c_size_t, [c_int, c_int]),
-    "mui_sample_filtered": (c_int, [_P, c_int, _P, c_long, c_int, c_int, _P, _P, c_float, _P, c_int, _P, c_float, _P, c_float, _P, _P, _P, ctypes.c_size_t]),
+    "mui_sample_filtered": (c_int, [_P, c_char_p]),  # packed by the Struct below
     "mui_probe_read": (c_int, [_P, _P, ctypes.c_uint64, _P]),
     "mui_tune_lock": (c_int, []),
     "mui_tune_gemv": (c_int, [c_int, c_int]),
@@ -209,6 +209,12 @@ class MuiChannelDeltaDesc(ctypes.Structure):
                                         "a_offset", "g_offset", "b_offset")]
                 + [("q_scale", c_float), ("epsilon", c_float)])
 
+
+# mui_paged_append_args, mui_paged_attention_args and mui_sample_filtered_args of the public header, member for member: packing one takes a tenth of what as many
+# ctypes arguments do, which counts beside kernels of a few microseconds. A NULL pointer is 0.
+PAGED_APPEND_ARGS = struct.Struct("13P7l12if0l")
+PAGED_ATTENTION_ARGS = struct.Struct("10PN3l13if0l")
+SAMPLE_FILTERED_ARGS = struct.Struct("9PNl4i3f0l")
 
 MUI_ABI_VERSION = 4  # MUI_ABI_VERSION of the public header: layout of the structs above
 

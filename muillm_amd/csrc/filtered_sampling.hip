@@ -454,31 +454,31 @@ extern "C" size_t mui_sample_filtered_workspace_bytes(int rows, int vocab) {
   return (size_t)rows * plan.parts * (131072 + 16);
 }
 
-extern "C" int mui_sample_filtered(mui_stream_t stream, int dtype, const void* logits, long row_stride, int rows, int vocab, const float* random_numbers,
-                                   const float* temperatures, float temperature, const int32_t* top_ks, int top_k, const float* top_ps, float top_p,
-                                   const float* min_ps, float min_p, int64_t* out_token, float* out_probability, void* workspace, size_t workspace_bytes) {
-  MUI_CHECK_ARG(logits && random_numbers && out_token && workspace && rows > 0 && vocab > 0 && row_stride >= vocab);
-  if (dtype != MUI_DTYPE_F16 && dtype != MUI_DTYPE_BF16) return MUI_ERR_INVALID_ARG;
-  if (rows > 65535 || vocab > kMostParts * kMostPart) return MUI_ERR_UNSUPPORTED;
-  if ((uintptr_t)workspace & 15u) return MUI_ERR_ALIGNMENT;
-  if (workspace_bytes < mui_sample_filtered_workspace_bytes(rows, vocab)) return MUI_ERR_INVALID_ARG;
-  const SamplePlan plan = sample_plan(rows, vocab);
+extern "C" int mui_sample_filtered(mui_stream_t stream, const mui_sample_filtered_args_t* args) {
+  MUI_CHECK_ARG(args);
+  const mui_sample_filtered_args_t& a = *args;
+  MUI_CHECK_ARG(a.logits && a.random_numbers && a.out_token && a.workspace && a.rows > 0 && a.vocab > 0 && a.row_stride >= a.vocab);
+  if (a.dtype != MUI_DTYPE_F16 && a.dtype != MUI_DTYPE_BF16) return MUI_ERR_INVALID_ARG;
+  if (a.rows > 65535 || a.vocab > kMostParts * kMostPart) return MUI_ERR_UNSUPPORTED;
+  if ((uintptr_t)a.workspace & 15u) return MUI_ERR_ALIGNMENT;
+  if (a.workspace_bytes < mui_sample_filtered_workspace_bytes(a.rows, a.vocab)) return MUI_ERR_INVALID_ARG;
+  const SamplePlan plan = sample_plan(a.rows, a.vocab);
   SampleParams p = {};
-  p.logits = (const uint16_t*)logits; p.row_stride = row_stride; p.rows = rows; p.vocab = vocab; p.parts = plan.parts; p.part_len = plan.part_len;
-  p.u = random_numbers;
-  p.temperature = temperatures; p.top_k = top_ks; p.top_p = top_ps; p.min_p = min_ps;
-  p.temperature1 = temperature; p.top_k1 = top_k; p.top_p1 = top_p; p.min_p1 = min_p;
-  p.counts = (uint16_t*)workspace;
-  p.runs = (unsigned long long*)((char*)workspace + (size_t)rows * plan.parts * 131072);
-  p.first = (uint32_t*)(p.runs + (size_t)rows * plan.parts);
-  p.token = out_token; p.share = out_probability;
+  p.logits = (const uint16_t*)a.logits; p.row_stride = a.row_stride; p.rows = a.rows; p.vocab = a.vocab; p.parts = plan.parts; p.part_len = plan.part_len;
+  p.u = a.random_numbers;
+  p.temperature = a.temperatures; p.top_k = a.top_ks; p.top_p = a.top_ps; p.min_p = a.min_ps;
+  p.temperature1 = a.temperature; p.top_k1 = a.top_k; p.top_p1 = a.top_p; p.min_p1 = a.min_p;
+  p.counts = (uint16_t*)a.workspace;
+  p.runs = (unsigned long long*)((char*)a.workspace + (size_t)a.rows * plan.parts * 131072);
+  p.first = (uint32_t*)(p.runs + (size_t)a.rows * plan.parts);
+  p.token = a.out_token; p.share = a.out_probability;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == MUI_DTYPE_F16) {
-    hipLaunchKernelGGL((sample_count_kernel<F16>), dim3(plan.parts, rows), dim3(kCountThreads), 0, s, p);
-    hipLaunchKernelGGL((sample_pick_kernel<F16>), dim3(rows), dim3(kCountThreads), 0, s, p);
+  if (a.dtype == MUI_DTYPE_F16) {
+    hipLaunchKernelGGL((sample_count_kernel<F16>), dim3(plan.parts, a.rows), dim3(kCountThreads), 0, s, p);
+    hipLaunchKernelGGL((sample_pick_kernel<F16>), dim3(a.rows), dim3(kCountThreads), 0, s, p);
   } else {
-    hipLaunchKernelGGL((sample_count_kernel<BF16>), dim3(plan.parts, rows), dim3(kCountThreads), 0, s, p);
-    hipLaunchKernelGGL((sample_pick_kernel<BF16>), dim3(rows), dim3(kCountThreads), 0, s, p);
+    hipLaunchKernelGGL((sample_count_kernel<BF16>), dim3(plan.parts, a.rows), dim3(kCountThreads), 0, s, p);
+    hipLaunchKernelGGL((sample_pick_kernel<BF16>), dim3(a.rows), dim3(kCountThreads), 0, s, p);
   }
   return launch_status();
 }

@@ -420,49 +420,47 @@ __global__ void __launch_bounds__(512) append_rows_kernel(const AppendParams p) 
 
 using namespace mui;
 
-extern "C" int mui_paged_append(mui_stream_t stream, int dtype, const void* q, long q_token_stride, long q_head_stride, const void* k, long k_token_stride,
-                                long k_head_stride, const void* v, long v_token_stride, long v_head_stride, void* k_pages, void* v_pages, float* k_scale,
-                                float* v_scale, int n_pages, int page_tokens, const int32_t* table, long table_stride, int table_pages, const int64_t* lengths,
-                                const int64_t* offsets, const int64_t* positions, const double* inv_freq, int rot_dim, int interleaved, float rope_scale,
-                                void* q_out, int n_rows, int n_requests, int max_tokens, int n_q_heads, int n_kv_heads, int head_dim) {
-  MUI_CHECK_ARG(k && v && k_pages && v_pages && k_scale && v_scale && table && lengths && (!q || q_out));
-  MUI_CHECK_ARG(n_pages > 0 && table_pages > 0 && table_stride >= table_pages && n_rows > 0 && n_requests > 0 && max_tokens > 0 && n_kv_heads > 0);
-  MUI_CHECK_ARG(!q || n_q_heads > 0);
-  MUI_CHECK_ARG(rot_dim >= 0 && rot_dim <= head_dim && (rot_dim == 0 || inv_freq));
-  MUI_CHECK_ARG(offsets || n_rows == n_requests);
-  if (dtype != MUI_DTYPE_F16 && dtype != MUI_DTYPE_BF16) return MUI_ERR_INVALID_ARG;
-  if (page_tokens != 64 && page_tokens != 128 && page_tokens != 256) return MUI_ERR_UNSUPPORTED;
-  if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || rot_dim % 16) return MUI_ERR_UNSUPPORTED;
-  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)q_out) & 15u) return MUI_ERR_ALIGNMENT;
-  if ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) return MUI_ERR_ALIGNMENT;
-  if (q && ((q_token_stride | q_head_stride) & 7)) return MUI_ERR_ALIGNMENT;
+extern "C" int mui_paged_append(mui_stream_t stream, const mui_paged_append_args_t* args) {
+  MUI_CHECK_ARG(args);
+  const mui_paged_append_args_t& a = *args;
+  MUI_CHECK_ARG(a.k && a.v && a.k_pages && a.v_pages && a.k_scale && a.v_scale && a.table && a.lengths && (!a.q || a.q_out));
+  MUI_CHECK_ARG(a.n_pages > 0 && a.table_pages > 0 && a.table_stride >= a.table_pages && a.n_rows > 0 && a.n_requests > 0 && a.max_tokens > 0 && a.n_kv_heads > 0);
+  MUI_CHECK_ARG(!a.q || a.n_q_heads > 0);
+  MUI_CHECK_ARG(a.rot_dim >= 0 && a.rot_dim <= a.head_dim && (a.rot_dim == 0 || a.inv_freq));
+  MUI_CHECK_ARG(a.offsets || a.n_rows == a.n_requests);
+  if (a.dtype != MUI_DTYPE_F16 && a.dtype != MUI_DTYPE_BF16) return MUI_ERR_INVALID_ARG;
+  if (a.page_tokens != 64 && a.page_tokens != 128 && a.page_tokens != 256) return MUI_ERR_UNSUPPORTED;
+  if ((a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) || a.rot_dim % 16) return MUI_ERR_UNSUPPORTED;
+  if (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.k_pages | (uintptr_t)a.v_pages | (uintptr_t)a.q_out) & 15u) return MUI_ERR_ALIGNMENT;
+  if ((a.k_token_stride | a.k_head_stride | a.v_token_stride | a.v_head_stride) & 7) return MUI_ERR_ALIGNMENT;
+  if (a.q && ((a.q_token_stride | a.q_head_stride) & 7)) return MUI_ERR_ALIGNMENT;
   AppendParams p = {};
-  p.q = (const uint16_t*)q; p.q_tok = q_token_stride; p.q_head = q_head_stride;
-  p.k = (const uint16_t*)k; p.k_tok = k_token_stride; p.k_head = k_head_stride;
-  p.v = (const uint16_t*)v; p.v_tok = v_token_stride; p.v_head = v_head_stride;
-  p.kp = (uint8_t*)k_pages; p.vp = (uint8_t*)v_pages; p.ks = k_scale; p.vs = v_scale;
-  p.positions = positions; p.inv_freq = inv_freq; p.q_out = (uint16_t*)q_out;
-  p.t = {table, table_stride, table_pages, lengths, offsets, n_requests, n_rows, n_pages, page_tokens == 64 ? 6 : page_tokens == 128 ? 7 : 8};
-  p.rope_scale = rope_scale; p.rot = rot_dim; p.interleaved = interleaved ? 1 : 0;
-  p.heads = q ? n_q_heads : 0; p.kv_heads = n_kv_heads; p.dim = head_dim;
+  p.q = (const uint16_t*)a.q; p.q_tok = a.q_token_stride; p.q_head = a.q_head_stride;
+  p.k = (const uint16_t*)a.k; p.k_tok = a.k_token_stride; p.k_head = a.k_head_stride;
+  p.v = (const uint16_t*)a.v; p.v_tok = a.v_token_stride; p.v_head = a.v_head_stride;
+  p.kp = (uint8_t*)a.k_pages; p.vp = (uint8_t*)a.v_pages; p.ks = a.k_scale; p.vs = a.v_scale;
+  p.positions = a.positions; p.inv_freq = a.inv_freq; p.q_out = (uint16_t*)a.q_out;
+  p.t = {a.table, a.table_stride, a.table_pages, a.lengths, a.offsets, a.n_requests, a.n_rows, a.n_pages, a.page_tokens == 64 ? 6 : a.page_tokens == 128 ? 7 : 8};
+  p.rope_scale = a.rope_scale; p.rot = a.rot_dim; p.interleaved = a.interleaved ? 1 : 0;
+  p.heads = a.q ? a.n_q_heads : 0; p.kv_heads = a.n_kv_heads; p.dim = a.head_dim;
   hipStream_t s = (hipStream_t)stream;
-  const int units = head_dim / 16;
-  if (max_tokens == 1) {
-    const long blocks = ((long)n_requests * (p.heads + 2 * n_kv_heads) * units + 255) / 256;
+  const int units = a.head_dim / 16;
+  if (a.max_tokens == 1) {
+    const long blocks = ((long)a.n_requests * (p.heads + 2 * a.n_kv_heads) * units + 255) / 256;
     if (blocks > 0x7fffffffL) return MUI_ERR_UNSUPPORTED;
-    if (dtype == MUI_DTYPE_F16)
+    if (a.dtype == MUI_DTYPE_F16)
       hipLaunchKernelGGL((append_step_kernel<F16>), dim3((unsigned)blocks), dim3(256), 0, s, p);
     else
       hipLaunchKernelGGL((append_step_kernel<BF16>), dim3((unsigned)blocks), dim3(256), 0, s, p);
     return launch_status();
   }
   // 32 values a thread, of the larger pages 64 and 128
-  const int values = page_tokens * head_dim / 32, threads = values < 512 ? values : 512;
+  const int values = a.page_tokens * a.head_dim / 32, threads = values < 512 ? values : 512;
   const long rows_per = threads / units;
-  const long q_blocks = q ? (n_rows + rows_per - 1) / rows_per * ((n_q_heads + kQueryHeads - 1) / kQueryHeads) : 0;
-  const long pages = (long)n_rows / page_tokens + 2 * (long)n_requests;  // that new tokens can lie in
-  p.at_once = pages * 2 * n_kv_heads > 1024 ? 2 : 1;
-  const long blocks = q_blocks + pages * 2 * ((n_kv_heads + p.at_once - 1) / p.at_once);
+  const long q_blocks = a.q ? (a.n_rows + rows_per - 1) / rows_per * ((a.n_q_heads + kQueryHeads - 1) / kQueryHeads) : 0;
+  const long pages = (long)a.n_rows / a.page_tokens + 2 * (long)a.n_requests;  // that new tokens can lie in
+  p.at_once = pages * 2 * a.n_kv_heads > 1024 ? 2 : 1;
+  const long blocks = q_blocks + pages * 2 * ((a.n_kv_heads + p.at_once - 1) / p.at_once);
   if (blocks > 0x7fffffffL) return MUI_ERR_UNSUPPORTED;
   p.q_blocks = (int)q_blocks;
   const dim3 grid((unsigned)blocks), block(threads);
@@ -472,6 +470,6 @@ extern "C" int mui_paged_append(mui_stream_t stream, int dtype, const void* q, l
     else if (values == 1024) hipLaunchKernelGGL((append_rows_kernel<TT, 2>), grid, block, 0, s, p);   \
     else hipLaunchKernelGGL((append_rows_kernel<TT, 4>), grid, block, 0, s, p);                       \
   } while (0)
-  if (dtype == MUI_DTYPE_F16) MUI_APPEND_GO(F16); else MUI_APPEND_GO(BF16);
+  if (a.dtype == MUI_DTYPE_F16) MUI_APPEND_GO(F16); else MUI_APPEND_GO(BF16);
   return launch_status();
 }

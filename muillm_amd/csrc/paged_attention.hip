@@ -1082,44 +1082,41 @@ extern "C" size_t mui_paged_attention_scratch_bytes(int n_rows, int n_requests, 
   return paged_plan(n_rows, n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads, head_dim).scratch;
 }
 
-extern "C" int mui_paged_attention(mui_stream_t stream, int dtype, const void* q, long q_token_stride, long q_head_stride, const void* k_pages,
-                                   const void* v_pages, const float* k_scale, const float* v_scale, int n_pages, int page_tokens, const int32_t* table,
-                                   long table_stride, int table_pages, const int64_t* lengths, const int64_t* offsets, float scale, int window, int keep_first,
-                                   int max_tokens, int max_length, void* scratch, size_t scratch_bytes, void* out, int n_rows, int n_requests, int n_q_heads,
-                                   int n_kv_heads, int head_dim) {
-  MUI_CHECK_ARG(q && k_pages && v_pages && k_scale && v_scale && table && lengths && out);
-  MUI_CHECK_ARG(paged_attention_sizes(n_rows, n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads, head_dim));
-  MUI_CHECK_ARG(n_pages > 0 && table_pages > 0 && table_stride >= table_pages && (offsets || n_rows == n_requests) && scale > 0.f);
-  if (dtype != MUI_DTYPE_F16 && dtype != MUI_DTYPE_BF16) return MUI_ERR_INVALID_ARG;
-  if (page_tokens != 64 && page_tokens != 128 && page_tokens != 256) return MUI_ERR_UNSUPPORTED;
-  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return MUI_ERR_UNSUPPORTED;
-  if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out | (uintptr_t)scratch) & 15u) return MUI_ERR_ALIGNMENT;
-  if ((q_token_stride | q_head_stride) & 7) return MUI_ERR_ALIGNMENT;
-  const long cap = (long)table_pages * page_tokens;
-  if (max_length > cap) max_length = (int)cap;
-  const PagedPlan plan = paged_plan(n_rows, n_requests, max_tokens, max_length, window, keep_first, n_q_heads, n_kv_heads, head_dim);
-  if (plan.scratch && (!scratch || scratch_bytes < plan.scratch)) return MUI_ERR_INVALID_ARG;
-  if ((long)n_rows * n_q_heads > 0x7fffffffL - 256) return MUI_ERR_UNSUPPORTED;
+extern "C" int mui_paged_attention(mui_stream_t stream, const mui_paged_attention_args_t* args) {
+  MUI_CHECK_ARG(args);
+  const mui_paged_attention_args_t& a = *args;
+  MUI_CHECK_ARG(a.q && a.k_pages && a.v_pages && a.k_scale && a.v_scale && a.table && a.lengths && a.out);
+  MUI_CHECK_ARG(paged_attention_sizes(a.n_rows, a.n_requests, a.max_tokens, a.max_length, a.window, a.keep_first, a.n_q_heads, a.n_kv_heads, a.head_dim));
+  MUI_CHECK_ARG(a.n_pages > 0 && a.table_pages > 0 && a.table_stride >= a.table_pages && (a.offsets || a.n_rows == a.n_requests) && a.scale > 0.f);
+  if (a.dtype != MUI_DTYPE_F16 && a.dtype != MUI_DTYPE_BF16) return MUI_ERR_INVALID_ARG;
+  if (a.page_tokens != 64 && a.page_tokens != 128 && a.page_tokens != 256) return MUI_ERR_UNSUPPORTED;
+  if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return MUI_ERR_UNSUPPORTED;
+  if (((uintptr_t)a.q | (uintptr_t)a.k_pages | (uintptr_t)a.v_pages | (uintptr_t)a.out | (uintptr_t)a.scratch) & 15u) return MUI_ERR_ALIGNMENT;
+  if ((a.q_token_stride | a.q_head_stride) & 7) return MUI_ERR_ALIGNMENT;
+  const long cap = (long)a.table_pages * a.page_tokens;
+  const PagedPlan plan = paged_plan(a.n_rows, a.n_requests, a.max_tokens, a.max_length < cap ? a.max_length : (int)cap, a.window, a.keep_first, a.n_q_heads, a.n_kv_heads, a.head_dim);
+  if (plan.scratch && (!a.scratch || a.scratch_bytes < plan.scratch)) return MUI_ERR_INVALID_ARG;
+  if ((long)a.n_rows * a.n_q_heads > 0x7fffffffL - 256) return MUI_ERR_UNSUPPORTED;
   const bool prompt = plan.block_cols > 16;
   const long blocks = plan.blocks;
-  if (blocks > 0x7fffffffL || plan.splits > 65535 || n_requests > 65535) return MUI_ERR_UNSUPPORTED;
+  if (blocks > 0x7fffffffL || plan.splits > 65535 || a.n_requests > 65535) return MUI_ERR_UNSUPPORTED;
   PagedAttnParams p = {};
-  p.q = (const uint16_t*)q; p.q_tok = q_token_stride; p.q_head = q_head_stride;
-  p.kp = (const uint8_t*)k_pages; p.vp = (const uint8_t*)v_pages; p.ks = k_scale; p.vs = v_scale;
-  p.t = {table, table_stride, table_pages, lengths, offsets, n_requests, n_rows, n_pages, page_tokens == 64 ? 6 : page_tokens == 128 ? 7 : 8};
-  p.scale = scale * 1.4426950408889634f;
-  p.window = window; p.keep = window > 0 ? keep_first : 0;
-  p.heads = n_q_heads; p.kv_heads = n_kv_heads; p.group = n_q_heads / n_kv_heads;
+  p.q = (const uint16_t*)a.q; p.q_tok = a.q_token_stride; p.q_head = a.q_head_stride;
+  p.kp = (const uint8_t*)a.k_pages; p.vp = (const uint8_t*)a.v_pages; p.ks = a.k_scale; p.vs = a.v_scale;
+  p.t = {a.table, a.table_stride, a.table_pages, a.lengths, a.offsets, a.n_requests, a.n_rows, a.n_pages, a.page_tokens == 64 ? 6 : a.page_tokens == 128 ? 7 : 8};
+  p.scale = a.scale * 1.4426950408889634f;
+  p.window = a.window; p.keep = a.window > 0 ? a.keep_first : 0;
+  p.heads = a.n_q_heads; p.kv_heads = a.n_kv_heads; p.group = a.n_q_heads / a.n_kv_heads;
   p.block_cols = plan.block_cols; p.col_tiles = plan.col_tiles; p.split_tiles = plan.split_tiles; p.splits = plan.splits;
-  if (plan.scratch && prompt) p.part = (float*)scratch;
+  if (plan.scratch && prompt) p.part = (float*)a.scratch;
   if (plan.scratch && !prompt) {
-    p.before = (int*)scratch;
-    p.part = (float*)((char*)scratch + (((size_t)n_requests + 1) * 4 + 255) / 256 * 256);
+    p.before = (int*)a.scratch;
+    p.part = (float*)((char*)a.scratch + (((size_t)a.n_requests + 1) * 4 + 255) / 256 * 256);
   }
-  p.out = (uint16_t*)out;
+  p.out = (uint16_t*)a.out;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(plan.workgroups ? plan.workgroups : blocks));
-  const dim3 join((unsigned)(((long)n_rows * n_q_heads + 3) / 4));
+  const dim3 join((unsigned)(((long)a.n_rows * a.n_q_heads + 3) / 4));
 #define MUI_PAGED_GO(TT, DC, PIECES)                                                                                                       \
   do {                                                                                                                                     \
     if (prompt) {                                                                                                                          \
@@ -1138,7 +1135,7 @@ extern "C" int mui_paged_attention(mui_stream_t stream, int dtype, const void* q
     }                                                                                                                                      \
   } while (0)
 #define MUI_PAGED_TYPES(DC) \
-  do { if (dtype == MUI_DTYPE_F16) MUI_PAGED_GO(F16, DC, 3); else MUI_PAGED_GO(BF16, DC, 2); } while (0)
-  if (head_dim == 64) MUI_PAGED_TYPES(1); else if (head_dim == 128) MUI_PAGED_TYPES(2); else MUI_PAGED_TYPES(4);
+  do { if (a.dtype == MUI_DTYPE_F16) MUI_PAGED_GO(F16, DC, 3); else MUI_PAGED_GO(BF16, DC, 2); } while (0)
+  if (a.head_dim == 64) MUI_PAGED_TYPES(1); else if (a.head_dim == 128) MUI_PAGED_TYPES(2); else MUI_PAGED_TYPES(4);
   return launch_status();
 }

@@ -1350,7 +1350,7 @@ def _sample_workspace_bytes(rows: int, vocab: int) -> int:
 def _per_row(value, name: str, rows: int, dtype: torch.dtype, index: int, off):
     """(pointer, number) of a setting given as one number or as a tensor of one per row."""
     if not isinstance(value, torch.Tensor):
-        return None, off if value is None else value
+        return 0, off if value is None else value
     if value.dtype is not dtype or value.numel() != rows or not value.is_contiguous() or value.get_device() != index:
         raise RuntimeError(f"{name} must be a number or a contiguous {dtype} tensor of {rows} on the logits' device")
     return value.data_ptr(), off
@@ -1376,7 +1376,7 @@ def mui_sample_filtered(logits: torch.Tensor, random_numbers: torch.Tensor, temp
     if rows > 1 and l2.stride(0) < v:
         l2 = l2.contiguous()
     us, _ = _per_row(random_numbers, "random_numbers", rows, f32, at, None)
-    if us is None:
+    if not us and rows:
         raise RuntimeError(f"random_numbers must be a contiguous {f32} tensor of {rows}")
     ts, t = _per_row(temperature, "temperature", rows, f32, at, 1.0)
     ks, k = _per_row(top_k, "top_k", rows, torch.int32, at, 0)
@@ -1389,10 +1389,11 @@ def mui_sample_filtered(logits: torch.Tensor, random_numbers: torch.Tensor, temp
     if rows == 0:
         return token, probability
     nbytes = _sample_workspace_bytes(rows, v)
-    workspace = l2.new_empty(nbytes, dtype=torch.uint8)
+    workspace = l2.new_empty(nbytes // 2)
+    args = _lib.SAMPLE_FILTERED_ARGS.pack(l2.data_ptr(), us, ts, ks, ps, ms, token.data_ptr(), probability.data_ptr(), workspace.data_ptr(), nbytes,
+                                          l2.stride(0) if rows > 1 else v, code, rows, v, k, t, p, m)
     with _HERE if at == torch._C._cuda_getDevice() else torch.cuda.device(at):
-        check(_lib.load().mui_sample_filtered(torch._C._cuda_getCurrentRawStream(at), code, l2.data_ptr(), l2.stride(0) if rows > 1 else v, rows, v, us, ts, t, ks, k, ps, p,
-                                              ms, m, token.data_ptr(), probability.data_ptr(), workspace.data_ptr(), nbytes), "mui_sample_filtered")
+        check(_lib.load().mui_sample_filtered(torch._C._cuda_getCurrentRawStream(at), args), "mui_sample_filtered")
     return token, probability
 
 

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import MUI_DTYPE_BF16, MUI_DTYPE_F16, check
+from ._lib import MUI_DTYPE_BF16, MUI_DTYPE_F16, PAGED_APPEND_ARGS, PAGED_ATTENTION_ARGS, check
 
 PAGE_TOKENS = (64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
@@ -39,9 +39,12 @@ class PagedKV:
         if page not in PAGE_TOKENS or dim not in HEAD_DIMS:
             raise RuntimeError(f"pages hold {PAGE_TOKENS} tokens and heads {HEAD_DIMS} dimensions, not {page} and {dim}")
         self.index = at = k.get_device()
-        for name, x, dtype in (("k", k, _E4M3), ("v", v, _E4M3), ("k_scale", k_scale, _F32), ("v_scale", v_scale, _F32)):
-            if x.dtype is not dtype or not x.is_contiguous() or x.get_device() != at:
-                raise RuntimeError(f"{name} must be a contiguous {dtype} tensor on {k.device}")
+        if not (k.dtype is _E4M3 and v.dtype is _E4M3 and k_scale.dtype is _F32 and v_scale.dtype is _F32):
+            raise RuntimeError("k and v must be float8_e4m3fn tensors, k_scale and v_scale float32 ones")
+        if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+            raise RuntimeError("k, v and their scales must be contiguous")
+        if v.get_device() != at or k_scale.get_device() != at or v_scale.get_device() != at:
+            raise RuntimeError(f"v and the scales must be on {k.device}, as k is")
         if k_scale.shape != (n, h) or v_scale.shape != (n, h):
             raise RuntimeError("k_scale and v_scale must be [pages, kv_heads]")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
@@ -70,18 +73,18 @@ class PagedKV:
 
 
 # (A step of small requests takes the GPU a few microseconds, so what the host does in front of it counts: the checks ask a tensor for its device's number, its
-# shape and its strides once, and the stream comes as the number that it is, not as an object.)
-def _call(index: int, fn, *args) -> int:
+# shape and its strides once, arguments go to the library in one piece, and the stream comes as the number that it is, not as an object.)
+def _call(index: int, fn, args: bytes) -> int:
     if index == torch._C._cuda_getDevice():
-        return fn(torch._C._cuda_getCurrentRawStream(index), *args)
+        return fn(torch._C._cuda_getCurrentRawStream(index), args)
     with torch.cuda.device(index):
-        return fn(torch._C._cuda_getCurrentRawStream(index), *args)
+        return fn(torch._C._cuda_getCurrentRawStream(index), args)
 
 
 def _rows(x: torch.Tensor, name: str, kv: PagedKV, heads: Optional[int], dtype: torch.dtype, n_rows: int):
     """[rows, heads, dim] with whole heads: its heads and its strides between tokens and heads."""
     s = x.shape
-    if x.get_device() != kv.index or not x.is_cuda:
+    if x.get_device() != kv.index:
         raise RuntimeError(f"{name} must be a CUDA tensor on the cache's device")
     if x.dtype is not dtype or len(s) != 3 or s[0] != n_rows or s[2] != kv.dim or (heads is not None and s[1] != heads):
         raise RuntimeError(f"{name} has shape {tuple(s)} and type {x.dtype}, expected {dtype} [{n_rows}, {heads or 'heads'}, {kv.dim}]")
@@ -93,8 +96,8 @@ def _rows(x: torch.Tensor, name: str, kv: PagedKV, heads: Optional[int], dtype: 
 
 def _places(kv: PagedKV, table: torch.Tensor, lengths: torch.Tensor, offsets: Optional[torch.Tensor], n_rows: int):
     """(requests, pages of a row of the table, from row to row)"""
-    if table.get_device() != kv.index or lengths.get_device() != kv.index or not table.is_cuda:
-        raise RuntimeError("table and lengths must be CUDA tensors on the cache's device")
+    if kv.index < 0 or table.get_device() != kv.index or lengths.get_device() != kv.index:
+        raise RuntimeError("table and lengths must be CUDA tensors on the cache's device, which is one")
     s = table.shape
     if table.dtype is not _I32 or len(s) != 2 or s[1] < 1:
         raise RuntimeError("table must be int32 [requests, pages]")
@@ -134,7 +137,7 @@ def _scratch_bytes(*sizes: int) -> int:
 
 def _output(out: Optional[torch.Tensor], q: torch.Tensor, in_place: bool) -> torch.Tensor:
     if out is None:
-        return q.new_empty(q.shape)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.dtype is not q.dtype or out.shape != q.shape or not out.is_contiguous() or out.get_device() != q.get_device():
         raise RuntimeError("out must be a contiguous tensor of q's shape and type")
     if in_place and out.data_ptr() == q.data_ptr() and q.is_contiguous():
@@ -167,7 +170,7 @@ def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, kv
     _, kt, kh = _rows(k, "k", kv, kv.kv_heads, dtype, n_rows)
     _, vt, vh = _rows(v, "v", kv, kv.kv_heads, dtype, n_rows)
     heads = qt = qh = 0
-    qp = op = fp = None
+    qp = op = fp = 0
     if q is not None:
         heads, qt, qh = _rows(q, "q", kv, None, dtype, n_rows)
         out = _output(out, q, True)
@@ -184,10 +187,11 @@ def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, kv
     if n_rows == 0:
         return out if q is not None else None
     max_tokens = _most_tokens(max_tokens, offsets, n_rows)
-    check(_call(kv.index, _lib.load().mui_paged_append, code, qp, qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, kv.k.data_ptr(), kv.v.data_ptr(),
-                kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.n_pages, kv.page, table.data_ptr(), step, width, lengths.data_ptr(),
-                None if offsets is None else offsets.data_ptr(), None if positions is None else positions.data_ptr(), fp, rot, 1 if interleaved else 0, rope_scale, op,
-                n_rows, n, max_tokens, heads, kv.kv_heads, kv.dim), "mui_paged_append")
+    args = PAGED_APPEND_ARGS.pack(qp, k.data_ptr(), v.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), table.data_ptr(),
+                                  lengths.data_ptr(), 0 if offsets is None else offsets.data_ptr(), 0 if positions is None else positions.data_ptr(), fp, op,
+                                  qt, qh, kt, kh, vt, vh, step,
+                                  code, kv.n_pages, kv.page, width, n_rows, n, max_tokens, heads, kv.kv_heads, kv.dim, rot, 1 if interleaved else 0, rope_scale)
+    check(_call(kv.index, _lib.load().mui_paged_append, args), "mui_paged_append")
     return out if q is not None else None
 
 
@@ -219,8 +223,9 @@ def paged_attention(q: torch.Tensor, kv: PagedKV, table: torch.Tensor, lengths: 
     most = min(width * kv.page, 0x7fffffff)
     max_length = most if max_length is None else max(1, min(max_length, most))
     nbytes = _scratch_bytes(n_rows, n, max_tokens, max_length, window, keep_first, heads, kv.kv_heads, kv.dim)
-    scratch = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    check(_call(kv.index, _lib.load().mui_paged_attention, code, q.data_ptr(), qt, qh, kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.n_pages,
-                kv.page, table.data_ptr(), step, width, lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), scale, window, keep_first, max_tokens, max_length,
-                None if scratch is None else scratch.data_ptr(), nbytes, out.data_ptr(), n_rows, n, heads, kv.kv_heads, kv.dim), "mui_paged_attention")
+    scratch = q.new_empty(nbytes // 2) if nbytes else None
+    args = PAGED_ATTENTION_ARGS.pack(q.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+                                     0 if offsets is None else offsets.data_ptr(), 0 if scratch is None else scratch.data_ptr(), out.data_ptr(), nbytes, qt, qh, step,
+                                     code, kv.n_pages, kv.page, width, n_rows, n, max_tokens, max_length, window, keep_first, heads, kv.kv_heads, kv.dim, scale)
+    check(_call(kv.index, _lib.load().mui_paged_attention, args), "mui_paged_attention")
     return out

@@ -1,4 +1,6 @@
 """The paged cache and its operators without a GPU: layouts, and calls that are refused before anything runs."""
+import re
+
 import pytest
 import torch
 
@@ -12,7 +14,8 @@ def append_args(**kw):
     a = dict(stream=None, dtype=0, q=P, qt=512, qh=128, k=P, kt=512, kh=128, v=P, vt=512, vh=128, kp=P, vp=P, ks=P, vs=P, n_pages=4, page=64, table=P, stride=2, pages=2,
              lengths=P, offsets=None, positions=None, inv_freq=P, rot=128, interleaved=0, factor=1.0, q_out=P, rows=2, requests=2, most=1, heads=4, kv_heads=2, dim=128)
     a.update(kw)
-    return list(a.values())
+    order = "q k v kp vp ks vs table lengths offsets positions inv_freq q_out qt qh kt kh vt vh stride dtype n_pages page pages rows requests most heads kv_heads dim rot interleaved factor"
+    return [a["stream"], _lib.PAGED_APPEND_ARGS.pack(*(a[x] or 0 for x in order.split()))]
 
 
 @pytest.mark.parametrize("change,status", [
@@ -30,7 +33,8 @@ def attention_args(**kw):
     a = dict(stream=None, dtype=0, q=P, qt=512, qh=128, kp=P, vp=P, ks=P, vs=P, n_pages=4, page=64, table=P, stride=2, pages=2, lengths=P, offsets=None, scale=0.1, window=0,
              keep=0, most=1, longest=128, scratch=None, nbytes=0, out=P, rows=2, requests=2, heads=4, kv_heads=2, dim=128)
     a.update(kw)
-    return list(a.values())
+    order = "q kp vp ks vs table lengths offsets scratch out nbytes qt qh stride dtype n_pages page pages rows requests most longest window keep heads kv_heads dim scale"
+    return [a["stream"], _lib.PAGED_ATTENTION_ARGS.pack(*(a[x] or 0 for x in order.split()))]
 
 
 @pytest.mark.parametrize("change,status", [
@@ -53,10 +57,11 @@ def test_scratch_of_bad_sizes_is_nothing():
 
 
 def sampling_args(**kw):
-    a = dict(stream=None, dtype=0, logits=P, stride=1000, rows=2, vocab=1000, u=P, ts=None, t=1.0, ks=None, k=0, ps=None, p=1.0, ms=None, m=0.0, token=P, probability=None,
+    a = dict(row_stream=None, dtype=0, logits=P, stride=1000, rows=2, vocab=1000, u=P, ts=None, t=1.0, ks=None, k=0, ps=None, p=1.0, ms=None, m=0.0, token=P, probability=None,
              ws=P, nbytes=1 << 40)
     a.update(kw)
-    return list(a.values())
+    order = "logits u ts ks ps ms token probability ws nbytes stride dtype rows vocab k t p m"
+    return [a["row_stream"], _lib.SAMPLE_FILTERED_ARGS.pack(*(a[x] or 0 for x in order.split()))]
 
 
 @pytest.mark.parametrize("change,status", [
@@ -119,3 +124,24 @@ def test_a_bound_above_the_rows_asks_for_no_more(dim, heads):
     for rows in (1, 7, 40, 200):
         one = lib.mui_paged_attention_scratch_bytes(rows, 4, rows, 5000, 0, 0, heads, 2, dim)
         assert one == lib.mui_paged_attention_scratch_bytes(rows, 4, 0x7fffffff, 5000, 0, 0, heads, 2, dim) < 1 << 30
+
+
+def test_the_packed_arguments_are_the_headers_structs():
+    """Numbers of members of each kind, in the header's order: pointers, sizes, longs, ints, floats."""
+    kinds = [("P", r"\*"), ("N", r"^size_t "), ("l", r"^long "), ("i", r"^int "), ("f", r"^float ")]
+    for name, packed in (("mui_paged_append_args", _lib.PAGED_APPEND_ARGS), ("mui_paged_attention_args", _lib.PAGED_ATTENTION_ARGS),
+                         ("mui_sample_filtered_args", _lib.SAMPLE_FILTERED_ARGS)):
+        body = re.search(r"typedef struct %s \{(.*?)\}" % name, _lib.header_text(), flags=re.S).group(1)
+        found = ""
+        for member in body.split(";"):
+            if member.strip():
+                kind = next(k for k, pattern in kinds if re.search(pattern, member.strip()))
+                found += kind * (member.count(",") + 1)
+        expanded = re.sub(r"(\d*)([A-Za-z])", lambda m: m.group(2) * int(m.group(1) or 1), packed.format)
+        assert found == expanded, name
+        assert packed.size % 8 == 0
+
+
+def test_no_arguments_are_refused():
+    lib = _lib.load()
+    assert lib.mui_paged_append(None, None) == lib.mui_paged_attention(None, None) == lib.mui_sample_filtered(None, None) == ARG
