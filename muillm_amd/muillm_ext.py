@@ -1389,8 +1389,8 @@ def mui_sample_filtered(logits: torch.Tensor, random_numbers: torch.Tensor, temp
     if rows == 0:
         return token, probability
     nbytes = _sample_workspace_bytes(rows, v)
-    workspace = l2.new_empty(nbytes // 2)
-    args = _lib.SAMPLE_FILTERED_ARGS.pack(l2.data_ptr(), us, ts, ks, ps, ms, token.data_ptr(), probability.data_ptr(), workspace.data_ptr(), nbytes,
+    workspace = l2.new_empty(nbytes // 2) if nbytes else None
+    args = _lib.SAMPLE_FILTERED_ARGS.pack(l2.data_ptr(), us, ts, ks, ps, ms, token.data_ptr(), probability.data_ptr(), 0 if workspace is None else workspace.data_ptr(), nbytes,
                                           l2.stride(0) if rows > 1 else v, code, rows, v, k, t, p, m)
     with _HERE if at == torch._C._cuda_getDevice() else torch.cuda.device(at):
         check(_lib.load().mui_sample_filtered(torch._C._cuda_getCurrentRawStream(at), args), "mui_sample_filtered")
