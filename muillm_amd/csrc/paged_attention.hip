@@ -1032,19 +1032,30 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
   PagedPlan r = {};
   if (max_tokens > n_rows) max_tokens = n_rows;
   const long group = n_q_heads / n_kv_heads;
-  const bool prompt = max_tokens * group > 64;
-  r.block_cols = prompt ? (head_dim == 256 ? 64 : 128) : 16;  // (256 dimensions: results of 32 columns a wave do not fit its registers)
-  r.col_tiles = (int)((max_tokens * group + r.block_cols - 1) / r.block_cols);
   long tiles = ((long)max_length + 63) / 64;
   if (window > 0) {
     const long seen = ((long)window + max_tokens + 62) / 64 + 1 + ((long)keep + 63) / 64;
     tiles = tiles < seen ? tiles : seen;
   }
   if (tiles < 1) tiles = 1;
-  // (of prompts: no more than the rows fill, and one of each request that is not full)
-  const long filled = ((long)n_rows * group + r.block_cols - 1) / r.block_cols + n_requests;
-  r.blocks = n_kv_heads * (prompt && filled < (long)n_requests * r.col_tiles ? filled : (long)n_requests * r.col_tiles);
-  const long units = r.blocks;
+  // Blocks of `per` columns of a request at most, and of all requests: no more than the rows fill, and one of each request that is not full.
+  auto each = [&](int per) { return (max_tokens * group + per - 1) / per; };
+  auto all = [&](int per) {
+    const long filled = (long)n_rows * group / per + n_requests, most = n_requests * each(per);
+    return filled < most ? filled : most;
+  };
+  const int wide = head_dim == 256 ? 64 : 128;  // (256 dimensions: results of 32 columns a wave do not fit its registers)
+  // The kernel for single tokens takes 2 ns for a block of 16 columns and a tile, the one for prompts 4 for a block of 128, and 6 us more to begin with and to join. us, the one / the other,
+  // 32 heads, 8 KV heads, 128 dimensions: one request of 1000 keys and 32 new tokens 12 / 23; of 8000 and 16 27 / 28, 32 35 / 30; 16 requests of 1000 and 16 24 / 31, 32 45 / 38; of 8000
+  // and 4 58 / 92, 8 97 / 85, 32 283 / 101.
+  const bool sparse = (long)n_requests * each(16) > 2 * all(16);  // a workgroup per unit would find most of them empty: those that begin and end take 8 ns each
+  const bool unit = !sparse && (tiles <= 16 || n_requests > kDealtRequests);
+  const bool dealt = !unit && n_requests <= kDealtRequests && (long)n_requests * each(16) <= 0x3fffffffL / tiles / n_kv_heads;
+  const bool prompt = !(unit || dealt) || (2 * all(16) - 3 * all(wide)) * n_kv_heads >= (12000 + tiles - 1) / tiles;
+  r.block_cols = prompt ? wide : 16;
+  r.col_tiles = (int)each(r.block_cols);
+  const long units = n_kv_heads * all(r.block_cols);
+  r.blocks = prompt ? units : (long)n_kv_heads * n_requests * r.col_tiles;
   r.splits = 1;
   r.split_tiles = (int)tiles;
   if (prompt) {
@@ -1060,7 +1071,7 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
   // 64 heads x 64 dimensions, 16 requests of 4096 keys 27.7 / 22.0; 128 dimensions, 32 requests of 200 to 4096 keys 35.5 / 40.7, 64 of 4096 to 16384 195.6 / 190.7.
   // 256 dimensions: a wave's registers are all of a SIMD's.
   r.waves = head_dim == 256 ? 4 : head_dim == 64 || tiles <= 16 || units * tiles >= 128 * 256 ? 8 : 4;
-  if (tiles <= 16 || n_requests > kDealtRequests || units * tiles > 0x3fffffffL) return r;  // a workgroup per unit
+  if (unit) return r;
   const long wanted = (units * tiles + r.waves - 1) / r.waves, most = head_dim == 256 || r.waves == 8 ? 256 : 512;
   r.workgroups = (int)(wanted < most ? wanted : most);
   r.scratch = (((size_t)n_requests + 1) * 4 + 255) / 256 * 256 + (size_t)r.workgroups * 2 * 16 * (head_dim + 4) * 4;

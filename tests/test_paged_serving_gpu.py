@@ -382,3 +382,12 @@ def test_prompts_of_many_requests(dtype, dim, page):
     run_attention(dtype, dim, page, lengths, new, 7, 1)
     run_attention(dtype, dim, page, lengths, new, 8, 2, max_tokens=90)
     run_attention(dtype, dim, page, lengths[:3] + [2000], [0, 0, 1, 300], 8, 1)
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(F16, 128, 64), (BF16, 64, 128), (BF16, 256, 64)])
+@pytest.mark.parametrize("requests,length,tokens", [(1, 300, 300), (1, 900, 33), (1, 2100, 17), (3, 1100, 9), (20, 130, 9), (2, 3000, 40)])
+def test_between_single_tokens_and_prompts(dtype, dim, page, requests, length, tokens):
+    """Either kernel, with and without a workgroup per block, around the sizes at which the other is taken."""
+    lengths = [max(tokens, length - 37 * b) for b in range(requests)]
+    run_attention(dtype, dim, page, lengths, [max(1, tokens - b) for b in range(requests)], 4, 2)
+    run_attention(dtype, dim, page, lengths, [tokens] + [0] * (requests - 1), 6, 1, window=100, keep=3)
