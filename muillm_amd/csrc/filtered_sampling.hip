@@ -489,13 +489,13 @@ struct SamplePlan { int parts, part_len; bool one; };
 static SamplePlan sample_plan(int rows, int vocab, int dtype) {
   SamplePlan r;
   // One workgroup a row, or several and a second launch. us, one / several: one row of 32000 bf16 logits 15.1 / 17.2, of 50000 18.9 / 17.5; 64 rows of 50000 20.4 / 20.4,
-  // 256 rows of 32000 17.3 / 23.0, of 65000 24.7 / 29.6.
-  r.one = vocab <= (rows < 64 ? 40000 : kMostPart);
+  // 256 rows of 32000 17.3 / 23.0, of 65000 24.7 / 29.6; fp16, one row of 50000 20.8 / 21.3, 16 rows 22.1 / 24.1.
+  r.one = vocab <= (rows < 64 && dtype == MUI_DTYPE_BF16 ? 40000 : kMostPart);
+  // Parts of 16384 tokens or more, no more workgroups than there are CUs (one's counts fill its LDS); of 32768 for fp16, whose counts of usual logits are 72 KB a part to add up
+  // (bf16's 10). us, 16384 / 32768: one row of 128256 bf16 logits 19.0 / 20.9, fp16 26.2 / 25.1, 16 rows of 200000 fp16 37.2 / 32.1.
   int parts = (vocab + kMostPart - 1) / kMostPart;
-  // Parts of 16384 tokens or more while there are CUs for them; of 32768 for fp16, whose counts of usual logits are 72 KB a part to add up (bf16's 10). us, 16384 / 32768: one
-  // row of 128256 bf16 logits 19.0 / 20.9, fp16 26.2 / 25.1, 16 rows of 200000 fp16 37.2 / 32.1.
   const int least = dtype == MUI_DTYPE_F16 ? 32768 : 16384;
-  const int want = (256 + rows - 1) / rows, most = (vocab + least - 1) / least;
+  const int want = rows < 256 ? 256 / rows : 1, most = (vocab + least - 1) / least;
   const int more = r.one ? 1 : want < most ? want : most;
   parts = parts > more ? parts : more;
   parts = parts < kMostParts ? parts : kMostParts;
