@@ -361,7 +361,9 @@ __device__ __forceinline__ RequestWork request_work(const PagedAttnParams& p, co
 // Single tokens, and several. A unit is 16 columns of one KV head and request. All tiles of all units, one after another, are dealt out to the workgroups in
 // equal shares, whatever the requests' lengths: the units that a share cuts are joined by a second launch. (Short caches: a workgroup per unit, nothing to join.) The waves of
 // a workgroup take every W-th tile each and meet in LDS. Two waves on a SIMD keep the memory busy, 16 KB on the way for each (128 dimensions): with the next tile requested
-// while one is worked on as well their registers do not suffice (64 requests of 4096 to 16384 tokens 204 instead of 190 us).
+// while one is worked on as well their registers do not suffice (64 requests of 4096 to 16384 tokens 204 instead of 187 us).
+// The cache's bytes bound it where there are many: those 64 requests, 8 KV heads of 128 dimensions (1.17 GB), 187 us, 6.2 TB/s; 32 requests of 200 to 4096 (90 MB) 29.6. With few it is the loads that
+// wait for one another (length, page, keys and values, again for each tile of a wave): 700 keys 9.4 us.
 template <typename T, int DC, int PIECES, int W>
 __global__ void __launch_bounds__(64 * W, DC == 4 ? W / 4 : 2) paged_columns_kernel(const PagedAttnParams p) {
   constexpr int D = DC * 64, kThreads = 64 * W;
@@ -498,7 +500,7 @@ __global__ void __launch_bounds__(64 * W, DC == 4 ? W / 4 : 2) paged_columns_ker
   }
 }
 
-// The units that shares have cut: a wave per row and head adds its parts up.
+// The units that shares have cut: a wave per row and head adds its parts up (4 us: where its parts begin, the parts, and the launch).
 template <typename T, int DC>
 __global__ void __launch_bounds__(256) paged_join_units_kernel(const PagedAttnParams p, int workgroups, int waves) {
   constexpr int D = DC * 64;
@@ -779,7 +781,10 @@ __device__ __forceinline__ bool nth_block(const PagedAttnParams& p, int n, int& 
 }
 
 // A workgroup of four waves takes 64 NT columns of one KV head (16 NT a wave) and `split_tiles` tiles, which its waves share through LDS: two tiles' room, the
-// next one's keys on their way to LDS and its values to registers while the waves work on one, one barrier a tile.
+// next one's keys on their way to LDS and its values to registers while the waves work on one, one barrier a tile. Two such workgroups on a CU (one of 256 dimensions).
+// 2048 tokens behind 6144, 32 query and 8 KV heads of 128 bf16 dimensions (240 GFLOP): 225 us, 1.07 PFLOP/s, 8-bit products of queries in two pieces and 16-bit ones of values; the matrix
+// instructions alone would take 117 us at the clock that the card keeps under them. Of the rest the tile's way through LDS is 59 us, exponentials 18, maxima 13, the barrier 9.
+// Eight waves that share a tile take 318, probabilities and values in 8 bits 340 us (100 vector instructions a tile more).
 template <typename T, int DC, int PIECES, int NT>
 __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const PagedAttnParams p) {
   constexpr int D = DC * 64, kCols = 64 * NT;
@@ -1059,8 +1064,11 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
   r.splits = 1;
   r.split_tiles = (int)tiles;
   if (prompt) {
-    long splits = (512 + units - 1) / units;
-    if (splits > (tiles + 7) / 8) splits = (tiles + 7) / 8;
+    // Keys divided among the workgroups that the card has room for at once, 8 tiles each at least. us with room for 256 / 512 / 1024: 100 new tokens of 4 requests of 8000 keys 104 / 84 / 93,
+    // 64 of one of 30000 66 / 65 / 89; tiles 8 / 16: 64 of one of 8000 35 / 39, 128 of two of 2000 30 / 37. The new tokens' own
+    // tiles count half, since as many are not seen: 1000 of one of 1000 takes 42 in two parts, 30 in one.
+    long splits = (head_dim == 256 ? 256 : 512) / units;
+    if (splits > (tiles - max_tokens / 128) / 8) splits = (tiles - max_tokens / 128) / 8;
     if (splits < 1) splits = 1;
     r.split_tiles = (int)((tiles + splits - 1) / splits);
     r.splits = (int)((tiles + r.split_tiles - 1) / r.split_tiles);
