@@ -826,7 +826,7 @@ int mui_channel_delta(mui_stream_t stream, int dtype, const mui_channel_delta_t*
  * The cache of one layer: pages of page_tokens (64, 128 or 256) tokens. k_pages: e4m3 codes [n_pages, n_kv_heads, page_tokens / 64, head_dim / 64, 64, 64], the last
  * two token and dimension. v_pages: e4m3 codes [n_pages, n_kv_heads, page_tokens / 64, head_dim, 4, 4, 4], the last three g, t, i of token 16 t + 4 g + i of the 64.
  * k_scale, v_scale: fp32 [n_pages, n_kv_heads], powers of two; a value is code * scale. head_dim 64, 128 or 256; pages, rows and outputs 16-byte aligned.
- * table: int32 [n_requests, table_pages], rows table_stride apart: a request's pages in order. lengths: int64 [n_requests], a request's tokens, the call's
+ * table: int32 [n_requests, table_pages], rows table_stride apart: a request's pages in order (fewer than 2^31 tokens of them). lengths: int64 [n_requests], a request's tokens, the call's
  * among them. offsets: int64 [n_requests + 1]: a request's new tokens are the rows offsets[b] .. offsets[b + 1] - 1 of the call's n_rows; NULL: row b (n_rows ==
  * n_requests). All of it on the device and read there. Whatever it holds, nothing outside the given buffers is read or written: an entry that is no page and places
  * beyond the table are left out, rows outside 0 .. n_rows do not exist. max_tokens (at least the most new tokens of a request) and max_length (at least the

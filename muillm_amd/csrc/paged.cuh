@@ -27,7 +27,9 @@ struct PagedTable {
 struct PagedSpan { int row0, count; long start, length; };
 __device__ __forceinline__ PagedSpan paged_span(const PagedTable& p, int b) {
   PagedSpan s;
+  constexpr long kMost = 1L << 36;  // (tiles of 64 tokens are counted in 32 bits)
   long len = p.lengths[b];
+  len = len < -kMost ? -kMost : (len > kMost ? kMost : len);
   const long cap = (long)p.pages << p.page_shift;
   long r0 = b, r1 = b + 1;
   if (p.offsets) { r0 = p.offsets[b]; r1 = p.offsets[b + 1]; }

@@ -438,6 +438,7 @@ extern "C" int mui_paged_append(mui_stream_t stream, const mui_paged_append_args
   if (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.k_pages | (uintptr_t)a.v_pages | (uintptr_t)a.q_out) & 15u) return MUI_ERR_ALIGNMENT;
   if ((a.k_token_stride | a.k_head_stride | a.v_token_stride | a.v_head_stride) & 7) return MUI_ERR_ALIGNMENT;
   if (a.q && ((a.q_token_stride | a.q_head_stride) & 7)) return MUI_ERR_ALIGNMENT;
+  if ((long)a.table_pages * a.page_tokens > 0x7fffffffL) return MUI_ERR_UNSUPPORTED;
   AppendParams p = {};
   p.q = (const uint16_t*)a.q; p.q_tok = a.q_token_stride; p.q_head = a.q_head_stride;
   p.k = (const uint16_t*)a.k; p.k_tok = a.k_token_stride; p.k_head = a.k_head_stride;

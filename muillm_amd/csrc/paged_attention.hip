@@ -1113,6 +1113,7 @@ extern "C" int mui_paged_attention(mui_stream_t stream, const mui_paged_attentio
   if (((uintptr_t)a.q | (uintptr_t)a.k_pages | (uintptr_t)a.v_pages | (uintptr_t)a.out | (uintptr_t)a.scratch) & 15u) return MUI_ERR_ALIGNMENT;
   if ((a.q_token_stride | a.q_head_stride) & 7) return MUI_ERR_ALIGNMENT;
   const long cap = (long)a.table_pages * a.page_tokens;
+  if (cap > 0x7fffffffL) return MUI_ERR_UNSUPPORTED;
   const PagedPlan plan = paged_plan(a.n_rows, a.n_requests, a.max_tokens, a.max_length < cap ? a.max_length : (int)cap, a.window, a.keep_first, a.n_q_heads, a.n_kv_heads, a.head_dim);
   if (plan.scratch && (!a.scratch || a.scratch_bytes < plan.scratch)) return MUI_ERR_INVALID_ARG;
   if ((long)a.n_rows * a.n_q_heads > 0x7fffffffL - 256) return MUI_ERR_UNSUPPORTED;

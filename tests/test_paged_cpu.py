@@ -22,7 +22,7 @@ def append_args(**kw):
     (dict(k=None), ARG), (dict(v=None), ARG), (dict(kp=None), ARG), (dict(vs=None), ARG), (dict(table=None), ARG), (dict(lengths=None), ARG), (dict(q_out=None), ARG),
     (dict(n_pages=0), ARG), (dict(pages=0), ARG), (dict(stride=1), ARG), (dict(rows=0), ARG), (dict(requests=0), ARG), (dict(most=0), ARG), (dict(kv_heads=0), ARG),
     (dict(heads=0), ARG), (dict(rot=-16), ARG), (dict(rot=144), ARG), (dict(inv_freq=None), ARG), (dict(rows=3), ARG), (dict(dtype=2), ARG), (dict(dtype=7), ARG),
-    (dict(page=32), UNSUPPORTED), (dict(page=96), UNSUPPORTED), (dict(page=512), UNSUPPORTED), (dict(dim=96, rot=64), UNSUPPORTED), (dict(rot=8), UNSUPPORTED),
+    (dict(page=32), UNSUPPORTED), (dict(page=96), UNSUPPORTED), (dict(pages=1 << 25, stride=1 << 25), UNSUPPORTED), (dict(page=512), UNSUPPORTED), (dict(dim=96, rot=64), UNSUPPORTED), (dict(rot=8), UNSUPPORTED),
     (dict(q=P + 2), ALIGNMENT), (dict(k=P + 8), ALIGNMENT), (dict(vp=P + 4), ALIGNMENT), (dict(kt=508), ALIGNMENT), (dict(vh=132), ALIGNMENT), (dict(qt=1), ALIGNMENT),
 ])
 def test_append_refusals(change, status):
@@ -41,7 +41,7 @@ def attention_args(**kw):
     (dict(q=None), ARG), (dict(kp=None), ARG), (dict(vp=None), ARG), (dict(ks=None), ARG), (dict(table=None), ARG), (dict(lengths=None), ARG), (dict(out=None), ARG),
     (dict(scale=0.0), ARG), (dict(scale=-1.0), ARG), (dict(scale=float("nan")), ARG), (dict(window=-1), ARG), (dict(keep=-1), ARG), (dict(most=0), ARG),
     (dict(longest=0), ARG), (dict(heads=5), ARG), (dict(heads=0), ARG), (dict(rows=0), ARG), (dict(rows=3), ARG), (dict(stride=1), ARG), (dict(dtype=2), ARG),
-    (dict(page=16), UNSUPPORTED), (dict(dim=192), UNSUPPORTED), (dict(requests=70000, rows=70000), UNSUPPORTED),
+    (dict(page=16), UNSUPPORTED), (dict(dim=192), UNSUPPORTED), (dict(pages=1 << 25, stride=1 << 25), UNSUPPORTED), (dict(requests=70000, rows=70000), UNSUPPORTED),
     (dict(q=P + 4), ALIGNMENT), (dict(out=P + 8), ALIGNMENT), (dict(kp=P + 1), ALIGNMENT), (dict(qh=4), ALIGNMENT),
     (dict(pages=2000, stride=2000, longest=100000), ARG),  # needs scratch and has none
 ])

@@ -391,3 +391,33 @@ def test_between_single_tokens_and_prompts(dtype, dim, page, requests, length, t
     lengths = [max(tokens, length - 37 * b) for b in range(requests)]
     run_attention(dtype, dim, page, lengths, [max(1, tokens - b) for b in range(requests)], 4, 2)
     run_attention(dtype, dim, page, lengths, [tokens] + [0] * (requests - 1), 6, 1, window=100, keep=3)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [9, 40, 3, 70]], ids=str)
+def test_lengths_that_are_none(new):
+    """Fewer tokens than are new, lengths beyond the table and any number that 64 bits hold: no token at a place that is none, and the requests beside them as ever."""
+    for window, keep in ((0, 0), (50, 5)):
+        for dtype, dim, page in ATTEND:
+            cache = Cache(9, 2, page, dim, 3)
+            table = torch.tensor([[0, 1], [2, 3], [4, 5], [6, 7]], dtype=torch.int32)
+            if max(new) > 1:
+                run_attention(dtype, dim, page, [5, 100, 1, 90], new, 4, 2, window, keep, table=table, cache=cache)
+            good = [90, 100, 80, 128]
+            want = None
+            for bad in (90, 1 << 62, -(1 << 63), (1 << 63) - 1, -7, 1 << 36, 1 << 32):
+                lengths = [good[0], bad, good[2], good[3]]
+                q = torch.randn((sum(new), 4, dim), generator=torch.Generator().manual_seed(2)).to(dtype).to(DEV)
+                x = q[:, :2].contiguous()
+                off = None if max(new) == 1 else offsets_of(new).to(DEV)
+                kv = cache.to_gpu()
+                ln = torch.tensor(lengths).to(DEV)
+                paged_ops.paged_append(None, x, x, kv, table.to(DEV), ln, off)
+                out = paged_ops.paged_attention(q, kv, table.to(DEV), ln, off, window=window, keep_first=keep).cpu()
+                rows = [r for b in (0, 2, 3) for r in range(sum(new[:b]), sum(new[:b + 1]))]
+                pages = [0, 1, 4, 5, 6, 7, 8]
+                got = (out[rows], kv.k.view(torch.uint8)[pages].cpu(), kv.v.view(torch.uint8)[pages].cpu())
+                want = want or got
+                assert all(torch.equal(a, b) for a, b in zip(got, want)), bad
+                if bad > 1000 or bad < 0:  # nothing of it was written
+                    untouched = cache.to_gpu()
+                    assert torch.equal(kv.k.view(torch.uint8)[2:4], untouched.k.view(torch.uint8)[2:4])
