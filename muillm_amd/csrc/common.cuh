@@ -196,6 +196,26 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// Inclusive sums over a wave, always in the same order: rows of 16 lanes by shifts, then the last lane of one to the rows behind it, in the vector ALU.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t n) { return n + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)n, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double w) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, w);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+  return w + __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+template <typename V>
+__device__ __forceinline__ V wave_scan(V x) {
+  x = dpp_add<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);  // row_bcast 15: rows 1, 3
+  return dpp_add<0x143, 0xc>(x);  // row_bcast 31: rows 2, 3
+}
+
 // Maximum / sum over the four 16-lane rows of a wave (lanes i, i + 16, i + 32, i + 48), the same
 // value in all four: gfx950's row-swap instructions exchange rows between two registers in the
 // vector ALU, without the LDS round trip of ds_bpermute that a shuffle by 16 or 32 lanes costs.

@@ -358,6 +358,13 @@ __device__ __forceinline__ RequestWork request_work(const PagedAttnParams& p, co
   return w;
 }
 
+// lane l's, in scalar registers
+__device__ __forceinline__ PagedSpan span_of_lane(const PagedSpan& s, int l) {
+  auto of = [l](int x) { return __builtin_amdgcn_readlane(x, l); };
+  auto of_long = [&](long x) { return (long)((unsigned long long)(uint32_t)of((int)(x >> 32)) << 32 | (uint32_t)of((int)(x & 0xffffffffL))); };
+  return {of(s.row0), of(s.count), of_long(s.start), of_long(s.length)};
+}
+
 // Single tokens, and several. A unit is 16 columns of one KV head and request. All tiles of all units, one after another, are dealt out to the workgroups in
 // equal shares, whatever the requests' lengths: the units that a share cuts are joined by a second launch. (Short caches: a workgroup per unit, nothing to join.) The waves of
 // a workgroup take every W-th tile each and meet in LDS. Two waves on a SIMD keep the memory busy, 16 KB on the way for each (128 dimensions): with the next tile requested
@@ -374,43 +381,55 @@ __global__ void __launch_bounds__(64 * W, DC == 4 ? W / 4 : 2) paged_columns_ker
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
   int b, unit = 0, tile0 = 0, share_begin = 0, share_end = 0, share = 0;
   if (p.part) {
-    int mine[kDealtRequests / kThreads], sum = 0;
-#pragma unroll
-    for (int k = 0; k < kDealtRequests / kThreads; ++k) {
-      const int r = threadIdx.x * (kDealtRequests / kThreads) + k;
-      if (r < p.t.n_requests) {
-        const RequestWork w = request_work(p, paged_span(p.t, r));
-        sum += w.tiles * w.blocks * p.kv_heads;
+    int to = 0;
+    const bool few = p.t.n_requests <= kWave;  // a request a lane, and every wave for itself
+    if (few) {
+      if (lane < p.t.n_requests) {
+        const RequestWork w = request_work(p, paged_span(p.t, lane));
+        to = w.tiles * w.blocks * p.kv_heads;
       }
-      mine[k] = sum;
-    }
-    int to = sum;
+      to = (int)wave_scan((uint32_t)to);
+      if (lane < p.t.n_requests) before[lane + 1] = to;  // (the same from all waves)
+    } else {
+      int mine[kDealtRequests / kThreads], sum = 0;
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(to, off);
-      if (lane >= off) to += o;
-    }
-    if (lane == 63) wave_sum[wave] = to;
-    __syncthreads();
-    int base = to - sum;
-    for (int w = 0; w < wave; ++w) base += wave_sum[w];
+      for (int k = 0; k < kDealtRequests / kThreads; ++k) {
+        const int r = threadIdx.x * (kDealtRequests / kThreads) + k;
+        if (r < p.t.n_requests) {
+          const RequestWork w = request_work(p, paged_span(p.t, r));
+          sum += w.tiles * w.blocks * p.kv_heads;
+        }
+        mine[k] = sum;
+      }
+      to = (int)wave_scan((uint32_t)sum);
+      if (lane == 63) wave_sum[wave] = to;
+      __syncthreads();
+      int base = to - sum;
+      for (int w = 0; w < wave; ++w) base += wave_sum[w];
 #pragma unroll
-    for (int k = 0; k < kDealtRequests / kThreads; ++k) before[threadIdx.x * (kDealtRequests / kThreads) + k + 1] = base + mine[k];
-    if (threadIdx.x == 0) before[0] = 0;
-    __syncthreads();
+      for (int k = 0; k < kDealtRequests / kThreads; ++k) before[threadIdx.x * (kDealtRequests / kThreads) + k + 1] = base + mine[k];
+      __syncthreads();
+    }
+    if (lane == 0) before[0] = 0;  // (of every wave, too)
     const int total = uniform(before[p.t.n_requests]);
-    share = share_of(total, gridDim.x, W);
-    if (blockIdx.x == 0)  // for the joining launch
-      for (int i = threadIdx.x; i <= p.t.n_requests; i += kThreads) p.before[i] = before[i];
+    share = uniform(share_of(total, gridDim.x, W));
+    if (blockIdx.x == 0)  // for the joining launch (of few requests by every wave, which has them all)
+      for (int i = few ? lane : threadIdx.x; i <= p.t.n_requests; i += few ? kWave : kThreads) p.before[i] = before[i];
     share_begin = (int)blockIdx.x * share;  // (share * workgroups < total + workgroups, which the host has checked)
     share_end = total - share_begin < share ? total : share_begin + share;
     if (share_begin >= total) return;
-    int lo = 0, hi = p.t.n_requests;  // the last request that begins at or before the share
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (before[mid] <= share_begin) lo = mid; else hi = mid;
+    // the last request that begins at or before the share
+    if (few) {
+      b = __ffsll((long long)__ballot(to > share_begin)) - 1;
+    } else {
+      int lo = 0, hi = p.t.n_requests;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (before[mid] <= share_begin) lo = mid; else hi = mid;
+      }
+      b = uniform(lo);
     }
-    b = uniform(lo);
+    unit = share_begin - uniform(before[b]);
   } else {
     unit = blockIdx.x % (p.kv_heads * p.col_tiles);
     b = blockIdx.x / (p.kv_heads * p.col_tiles);
@@ -419,8 +438,9 @@ __global__ void __launch_bounds__(64 * W, DC == 4 ? W / 4 : 2) paged_columns_ker
   RequestWork work = request_work(p, sp);
   int done = share_begin;
   if (p.part) {
-    unit = (done - uniform(before[b])) / work.tiles;
-    tile0 = done - uniform(before[b]) - unit * work.tiles;
+    const int in = unit;
+    unit = uniform(in / work.tiles);
+    tile0 = in - unit * work.tiles;
   } else if (unit >= work.blocks * p.kv_heads) {
     return;
   }
@@ -730,7 +750,6 @@ template <int PER>
 __device__ __forceinline__ bool nth_block(const PagedAttnParams& p, int n, int& b, int& block, PagedSpan& sp) {
   const int lane = threadIdx.x & 63;
   auto of = [](int x, int l) { return __builtin_amdgcn_readlane(x, l); };
-  auto of_long = [&](long x, int l) { return (long)((unsigned long long)(uint32_t)of((int)(x >> 32), l) << 32 | (uint32_t)of((int)(x & 0xffffffffL), l)); };
   for (int r0 = 0; r0 < p.t.n_requests; r0 += kWave) {
     PagedSpan s = {};
     int blocks = 0, top = 0;
@@ -774,7 +793,7 @@ __device__ __forceinline__ bool nth_block(const PagedAttnParams& p, int n, int& 
     const int l = __ffsll((long long)__ballot((at >> lane & 1ull) && __popcll(at & ((1ull << lane) - 1ull)) == n)) - 1;
     b = r0 + l;
     block = of(blocks - 1 - down, l);
-    sp = {of(s.row0, l), of(s.count, l), of_long(s.start, l), of_long(s.length, l)};
+    sp = span_of_lane(s, l);
     return true;
   }
   return false;
