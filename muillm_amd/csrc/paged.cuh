@@ -53,6 +53,21 @@ __device__ __forceinline__ int request_of(const PagedTable& t, int row) {
   return lo;
 }
 
+// the same for a row that a whole wave asks for, 64 requests looked at at once
+__device__ __forceinline__ int request_of_wave(const PagedTable& t, int row) {
+  if (!t.offsets) return row;
+  const int lane = threadIdx.x & 63;
+  int lo = 0, len = t.n_requests;
+  while (len > 1) {
+    const int step = (len + kWave - 1) / kWave, at = lane * step;
+    const unsigned long long in = __ballot(at < len && t.offsets[lo + (at < len ? at : 0)] <= row);
+    const int k = in ? (63 - __clzll((long long)in)) * step : 0;
+    lo += k;
+    len = len - k < step ? len - k : step;
+  }
+  return lo;
+}
+
 // (what a request's numbers say is the same for a workgroup, which the compiler does not see where they come from memory: in scalar registers it costs the results no room)
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ long uniform(long x) {

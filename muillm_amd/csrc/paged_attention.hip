@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(256) paged_join_units_kernel(const PagedAttnPa
   const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (item >= (long)p.t.n_rows * p.heads) return;
   const int row = (int)(item / p.heads), head = (int)(item % p.heads);
-  const int b = request_of(p.t, row);
+  const int b = request_of_wave(p.t, row);
   const PagedSpan sp = paged_span(p.t, b);
   if (row < sp.row0 || row >= sp.row0 + sp.count) return;
   const int col = (row - sp.row0) * p.group + head % p.group;
@@ -1028,7 +1028,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (item >= n) return;
   const int row = (int)(item / p.heads), head = (int)(item % p.heads);
-  const int b = request_of(p.t, row);
+  const int b = request_of_wave(p.t, row);
   const PagedSpan sp = paged_span(p.t, b);
   if (row < sp.row0 || row >= sp.row0 + sp.count) return;
   const int col = (row - sp.row0) * p.group + head % p.group;

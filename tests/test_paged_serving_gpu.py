@@ -421,3 +421,56 @@ def test_lengths_that_are_none(new):
                 if bad > 1000 or bad < 0:  # nothing of it was written
                     untouched = cache.to_gpu()
                     assert torch.equal(kv.k.view(torch.uint8)[2:4], untouched.k.view(torch.uint8)[2:4])
+
+
+@pytest.mark.parametrize("dtype,rows,vocab", [(BF16, 3, 70001), (F16, 2, 131072), (BF16, 70, 66000), (F16, 5, 8000)])
+def test_captured_sampling_of_one_and_two_launches(dtype, rows, vocab):
+    """Replays on other logits and numbers, eager calls between them: each the eager call's tokens and probabilities."""
+    g = torch.Generator().manual_seed(2)
+    given = [((2 * torch.randn((rows, vocab), generator=g)).to(dtype).to(DEV), torch.rand(rows, generator=g).to(DEV)) for _ in range(4)]
+    kw = dict(temperature=0.9, top_k=3000, top_p=0.95, min_p=1e-4)
+    want = [muillm_ext.mui_sample_filtered(x, u, **kw) for x, u in given]
+    logits, numbers = given[0][0].clone(), given[0][1].clone()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = muillm_ext.mui_sample_filtered(logits, numbers, **kw)
+        graphs.append((graph, out))
+    for i in range(8):
+        graph, out = graphs[i % 2]
+        logits.copy_(given[i % 4][0])
+        numbers.copy_(given[i % 4][1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[i % 4][0]) and torch.equal(out[1], want[i % 4][1]), f"replay {i}"
+        again = muillm_ext.mui_sample_filtered(given[(i + 1) % 4][0], given[(i + 1) % 4][1], **kw)
+        assert torch.equal(again[0], want[(i + 1) % 4][0])
+
+
+def test_captured_prompts_and_joined_results():
+    """Prompts whose keys are divided, and single tokens of long caches, replayed as the device's lengths change."""
+    page, heads, kv_heads, dim = 128, 8, 2, 128
+    cache = Cache(44, kv_heads, page, dim, 1)
+    kv = cache.to_gpu()
+    table = make_table([2600, 2700], page, 44, 0).to(DEV)
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn((48, heads, dim), generator=g).to(BF16).to(DEV)
+    off = torch.tensor([0, 40, 48], device=DEV)
+    lengths = torch.tensor([2000, 1500], device=DEV)
+
+    def calls():
+        return (paged_ops.paged_attention(q, kv, table, lengths, off, max_tokens=40), paged_ops.paged_attention(q[:2], kv, table, lengths))
+
+    calls()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = calls()
+    for n in ([2000, 1500], [2600, 8], [41, 2700], [500, 900], [2000, 1500]):
+        lengths.copy_(torch.tensor(n))
+        graph.replay()
+        torch.cuda.synchronize()
+        again = calls()
+        assert torch.equal(out[0], again[0]) and torch.equal(out[1], again[1]), n
+        want, bound = attention(cache, q[:2].cpu(), table.cpu(), n, [1, 1], dim ** -0.5)
+        check(out[1], want, bound, str(n))
