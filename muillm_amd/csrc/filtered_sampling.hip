@@ -51,13 +51,14 @@ __device__ __forceinline__ void count_tokens(const uint16_t* x, int begin, int e
     const uint32_t k = place_of<T>(bits);
     if (k != 0xffffffffu) atomicAdd(&words[at(k >> 1)], 1u << (16 * (k & 1)));
   };
-  const bool vec = ((uintptr_t)(x + begin) & 15u) == 0;
-  const int whole = vec && end > begin ? (end - begin) >> 3 : 0;
+  // (rows begin anywhere: 16 bytes at a time from the first place that is aligned)
+  const int head = (int)(0u - (uint32_t)((uintptr_t)(x + begin) >> 1)) & 7;
+  const int first = begin + head < end ? begin + head : end, whole = end > first ? (end - first) >> 3 : 0;
   constexpr int kAhead = 4;
   for (int c0 = t; c0 < whole; c0 += kAhead * kCountThreads) {
     u32x4 v[kAhead];
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a) v[a] = ld16(x + begin + 8 * (c0 + a * kCountThreads < whole ? c0 + a * kCountThreads : c0));
+    for (int a = 0; a < kAhead; ++a) v[a] = ld16(x + first + 8 * (c0 + a * kCountThreads < whole ? c0 + a * kCountThreads : c0));
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
       if (c0 + a * kCountThreads >= whole) break;
@@ -68,7 +69,8 @@ __device__ __forceinline__ void count_tokens(const uint16_t* x, int begin, int e
       }
     }
   }
-  for (int i = begin + 8 * whole + t; i < end; i += kCountThreads) count(x[i]);
+  if (begin + t < first) count(x[begin + t]);
+  if (first + 8 * whole + t < end) count(x[first + 8 * whole + t]);
 }
 
 // One row of 128256 bf16 logits: 5.3 us here, 12.0 in sample_pick_kernel, of those 1.2 until the runs are known, 2.3 adding counts up, 2.1 weights, 2.2 the filters.
@@ -326,23 +328,22 @@ __device__ __forceinline__ void sample_token(const SampleParams& p, SampleShared
   const int part = sh.part;
   const uint16_t* x = p.logits + (long)row * p.row_stride;
   const int begin = part * p.part_len, end = begin + p.part_len < p.vocab ? begin + p.part_len : p.vocab;
-  const int per = ((p.part_len >> 3) + kWaves - 1) / kWaves * 8;  // tokens of a wave, at most 4096
-  const int wb = begin + wave * per, we = wb + per < end ? wb + per : end;
-  const bool vec = ((uintptr_t)(x + wb) & 15u) == 0;
+  const int per = ((p.part_len + 7) / 8 + kWaves) / kWaves * 8;  // tokens of a wave, at most 4096; one chunk of 8 more where the part begins within one
+  const int wb = begin - (int)((uintptr_t)(x + begin) >> 1 & 7) + wave * per, we = wb + per < end ? wb + per : end;
   unsigned long long found = 0;
 #pragma unroll 4
   for (int s = 0; s < 8; ++s) {
     const int i = wb + 512 * s + 8 * lane;
     if (i >= we) break;
     uint32_t m = 0;
-    if (i + 8 <= we && vec) {
+    if (i >= begin && i + 8 <= we) {
       const u32x4 v = ld16(x + i);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         m |= ((v[j] & 0xffffu) == bits || (v[j] & 0xffffu) == or_bits ? 1u : 0u) << (2 * j) | (v[j] >> 16 == bits || v[j] >> 16 == or_bits ? 2u : 0u) << (2 * j);
     } else {
       for (int j = 0; j < 8; ++j)
-        if (i + j < we) m |= (x[i + j] == bits || x[i + j] == or_bits ? 1u : 0u) << j;
+        if (i + j >= begin && i + j < we) m |= (x[i + j] == bits || x[i + j] == or_bits ? 1u : 0u) << j;
     }
     found |= (unsigned long long)m << (8 * s);
   }

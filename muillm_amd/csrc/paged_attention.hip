@@ -1073,7 +1073,9 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
   // 32 heads, 8 KV heads, 128 dimensions: one request of 1000 keys and 32 new tokens 12 / 23; of 8000 and 16 27 / 28, 32 35 / 30; 16 requests of 1000 and 16 24 / 31, 32 45 / 38; of 8000
   // and 4 58 / 92, 8 97 / 85, 32 283 / 101.
   const bool sparse = (long)n_requests * each(16) > 2 * all(16);  // a workgroup per unit would find most of them empty: those that begin and end take 8 ns each
-  const bool unit = !sparse && (tiles <= 16 || n_requests > kDealtRequests);
+  // A workgroup per unit needs no scan and no joining launch. us, a unit each / dealt out, 8 KV heads, requests of equal lengths, which suit it best: 64 dimensions, 8 requests of 1400 keys
+  // 12.3 / 15.6; 128 dimensions, one of 1400 17.2 / 16.0, 30 20.9 / 23.6, one of 2000 20.0 / 14.4, 30 26.3 / 31.6; 256 dimensions, 30 of 800 25.1 / 28.0, 8 of 1400 27.6 / 23.6.
+  const bool unit = !sparse && (tiles <= (head_dim == 256 ? 16 : 24) || n_requests > kDealtRequests);
   const bool dealt = !unit && n_requests <= kDealtRequests && (long)n_requests * each(16) <= 0x3fffffffL / tiles / n_kv_heads;
   const bool prompt = !(unit || dealt) || (2 * all(16) - 3 * all(wide)) * n_kv_heads >= (12000 + tiles - 1) / tiles;
   r.block_cols = prompt ? wide : 16;
@@ -1097,7 +1099,7 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
   // Eight waves to a workgroup and one workgroup to a CU, or four and two: eight cut fewer units, four have more of them at work where the shares are small. us, four / eight:
   // 64 heads x 64 dimensions, 16 requests of 4096 keys 27.7 / 22.0; 128 dimensions, 32 requests of 200 to 4096 keys 35.5 / 40.7, 64 of 4096 to 16384 195.6 / 190.7.
   // 256 dimensions: a wave's registers are all of a SIMD's.
-  r.waves = head_dim == 256 ? 4 : head_dim == 64 || tiles <= 16 || units * tiles >= 128 * 256 ? 8 : 4;
+  r.waves = head_dim == 256 ? 4 : head_dim == 64 || unit || units * tiles >= 128 * 256 ? 8 : 4;
   if (unit) return r;
   const long wanted = (units * tiles + r.waves - 1) / r.waves, most = head_dim == 256 || r.waves == 8 ? 256 : 512;
   r.workgroups = (int)(wanted < most ? wanted : most);

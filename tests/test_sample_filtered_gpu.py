@@ -161,3 +161,22 @@ def test_draws_follow_the_weights():
     seen = torch.bincount(token.cpu(), minlength=6).double()
     assert bool(((seen - n * w).abs() <= 1.0).all())
     assert torch.allclose(share.cpu().double(), w[token.cpu()], rtol=2.0 ** -23, atol=0)
+
+
+@pytest.mark.parametrize("dtype,vocab", [(F16, 9), (BF16, 1003), (F16, 47723), (BF16, 65521), (BF16, 70003)])
+def test_rows_that_begin_anywhere(dtype, vocab):
+    """Rows an odd number of logits apart, in a tensor that begins at any of eight places: each token at the ends of its row is found."""
+    logits, u = noise(9, vocab, dtype, 5)
+    for shift in (0, 1, 5):
+        wide = torch.full((9 * (vocab + 2) + 16,), 60.0, dtype=dtype, device=DEV)
+        at = wide[shift:shift + 9 * (vocab + 2)].view(9, vocab + 2)[:, :vocab]
+        at.copy_(logits)
+        token, _ = muillm_ext.mui_sample_filtered(at, u.to(DEV), temperature=0.9, top_p=0.95)
+        for r in range(9):
+            assert int(token[r]) == pick(logits[r], float(u[r]), torch.tensor(0.9).item(), 0, torch.tensor(0.95).item(), 0.0)[0]
+        for place in (0, 1, 7, 8, vocab - 8, vocab - 2, vocab - 1):
+            if 0 <= place < vocab:
+                one = logits.clone()
+                one[:, place] = 50.0
+                at.copy_(one)
+                assert muillm_ext.mui_sample_filtered(at, u.to(DEV), top_k=1)[0].tolist() == [place] * 9
