@@ -272,12 +272,14 @@ __device__ __forceinline__ int page_exponent(const AppendParams& p, float most, 
   return e;
 }
 
-// A page of a head is 32 values a thread (64 and 128 of the larger ones), which it holds between finding the largest and writing the codes. Keys: units of a token, as queries.
-// Values: 8 dimensions of four tokens 4 q .. 4 q + 3, whose codes are a dword of each dimension's row.
+// A page of a head is 32 IT values a thread, which it holds between finding the largest and writing the codes. Keys: units of a token, as queries. Values: 8 dimensions of four tokens
+// 4 q .. 4 q + 3, whose codes are a dword of each dimension's row. Where larger pages are filled as a rule a workgroup has 1024 threads (256 tokens of 256 dimensions: 512, and IT is 4);
+// few tokens in one of them are the work of 512 for that part of the page (several parts are read twice, for the largest and for the codes). us, 128 dimensions, pages of 256, the whole
+// page held / parts: 64 requests' 5 new tokens 28 / 19, 100 63 / 42; 8 requests' 1000 50 / 54; 256 dimensions, 8 requests' 500 52 / 76.
 // Bytes bound it: every query, key and value is read once and written once. 11500 tokens of 32 + 8 + 8 heads of 128 bf16 dimensions (213 MB) 48.8 us, 4.4 TB/s; a copy of 2 GiB reaches 4.95.
 // In the same launch queries fill the time in which pages wait for their largest value.
 template <typename T, int IT>
-__global__ void __launch_bounds__(512) append_rows_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(IT == 1 ? 1024 : 512) append_rows_kernel(const AppendParams p) {
   __shared__ float red[16];
   if ((int)blockIdx.x < p.q_blocks) {
     append_queries<T>(p, blockIdx.x);
@@ -319,103 +321,152 @@ __global__ void __launch_bounds__(512) append_rows_kernel(const AppendParams p) 
   if (b < 0) return;
   const PagedSpan sp = uniform(paged_span(p.t, b));
   const long first = sp.start < 0 ? 0 : sp.start;
-  {
-    const int page = paged_page(p.t, b, (int)slot);
-    if (page < 0) return;
-    const long low = first > slot * P ? first : slot * P;
-    const long end = sp.length < (slot + 1) * P ? sp.length : (slot + 1) * P;
-    const int at0 = (int)(low - slot * P), at1 = (int)(end - slot * P);
-    if (at1 <= at0) return;
-    const int row0 = sp.row0 + (int)(low - sp.start) - at0;  // of the page's first place
-    if (!values) {
-      constexpr bool kHeld = IT == 1;  // angles for all heads (of a larger page there are too many to hold)
-      float c[kHeld ? 2 : 1][8], s[kHeld ? 2 : 1][8];
+  const int page = paged_page(p.t, b, (int)slot);
+  if (page < 0) return;
+  const long low = first > slot * P ? first : slot * P;
+  const long end = sp.length < (slot + 1) * P ? sp.length : (slot + 1) * P;
+  const int at0 = (int)(low - slot * P), at1 = (int)(end - slot * P);
+  if (at1 <= at0) return;
+  const int row0 = sp.row0 + (int)(low - sp.start) - at0;  // of the page's first place
+  const int part_tokens = IT == 1 ? 2 * threads / units : P, part0 = IT == 1 ? at0 / part_tokens : 0, part1 = IT == 1 ? (at1 - 1) / part_tokens : 0;
+  constexpr int kHeads = 2;  // at_once, at most
+  const long head_bytes = (long)p.dim << p.t.page_shift;
+  if (!values) {
+    // this thread's units of a part: the cosines and sines of their tokens (of more than two there are too many to hold), then, turned, a head's
+    float c[2][8], s[2][8];
+    auto angles = [&](int part) {
 #pragma unroll
-      for (int k = 0; k < (kHeld ? 2 : 0); ++k) {
-        const int j = threadIdx.x + k * threads, u = j % units, at = j / units;
-        const Unit n = unit_of(p, u);
+      for (int k = 0; k < (IT == 1 ? 2 : 0); ++k) {
+        const int j = threadIdx.x + k * threads, at = part * part_tokens + j / units;
+        const Unit n = unit_of(p, j % units);
         if (at >= at0 && at < at1 && n.turns0) unit_angles(p, n, (double)(p.positions ? p.positions[row0 + at] : slot * P + at), c[k], s[k]);
       }
+    };
+    float x[2 * IT][16];
+    auto take = [&](int part, int h) {
+      float most = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2 * IT; ++k) {
+        const int j = threadIdx.x + k * threads, at = part * part_tokens + j / units;
+        if (at >= at0 && at < at1) {
+          const Unit n = unit_of(p, j % units);
+          load_unit<T>(p.k + (long)(row0 + at) * p.k_tok + (long)h * p.k_head, n.d0, n.d1, x[k]);
+          if constexpr (IT > 1) {
+            if (n.turns0) unit_angles(p, n, (double)(p.positions ? p.positions[row0 + at] : slot * P + at), c[0], s[0]);
+          }
+          if (n.turns0) unit_turn(p, n, c[IT == 1 ? k : 0], s[IT == 1 ? k : 0], x[k]);
+#pragma unroll
+          for (int m = 0; m < 16; ++m) most = fmaxf(most, finite_abs(x[k][m]));
+        }
+      }
+      return most;
+    };
+    auto put = [&](int part, uint8_t* base, float inv) {
+#pragma unroll
+      for (int k = 0; k < 2 * IT; ++k) {
+        const int j = threadIdx.x + k * threads, at = part * part_tokens + j / units;
+        if (at >= at0 && at < at1) {
+          const Unit n = unit_of(p, j % units);
+          uint32_t w[4];
+#pragma unroll
+          for (int m = 0; m < 4; ++m) w[m] = to_e4m3x4(x[k][4 * m] * inv, x[k][4 * m + 1] * inv, x[k][4 * m + 2] * inv, x[k][4 * m + 3] * inv);
+          *(u32x2*)(base + k_at(p.dim, at, n.d0)) = u32x2{w[0], w[1]};
+          *(u32x2*)(base + k_at(p.dim, at, n.d1)) = u32x2{w[2], w[3]};
+        }
+      }
+    };
+    auto scaled = [&](int h, float most, float before_s) {
+      const long ph = (long)page * p.kv_heads + h;
+      __syncthreads();  // (red)
+      return exp2i(-page_exponent(p, block_most(most, red), p.kp + ph * head_bytes, p.ks + ph, before_s, at0, false));
+    };
+    if (IT > 1 || part0 == part1) {
+      angles(part0);
       for (int h = h0; h < h1; ++h) {
         const long ph = (long)page * p.kv_heads + h;
-        uint8_t* base = p.kp + ph * ((long)p.dim << p.t.page_shift);
-        const float before_s = p.ks[ph];
-        float most = 0.f, x[2 * IT][16];
-#pragma unroll
-        for (int k = 0; k < 2 * IT; ++k) {
-          const int j = threadIdx.x + k * threads, u = j % units, at = j / units;
-          if (at >= at0 && at < at1) {
-            const Unit n = unit_of(p, u);
-            load_unit<T>(p.k + (long)(row0 + at) * p.k_tok + (long)h * p.k_head, n.d0, n.d1, x[k]);
-            if (n.turns0) {
-              if constexpr (!kHeld) unit_angles(p, n, (double)(p.positions ? p.positions[row0 + at] : slot * P + at), c[0], s[0]);
-              unit_turn(p, n, c[kHeld ? k : 0], s[kHeld ? k : 0], x[k]);
-            }
-#pragma unroll
-            for (int m = 0; m < 16; ++m) most = fmaxf(most, finite_abs(x[k][m]));
-          }
-        }
-        __syncthreads();  // (red)
-        const float inv = exp2i(-page_exponent(p, block_most(most, red), base, p.ks + ph, before_s, at0, false));
-#pragma unroll
-        for (int k = 0; k < 2 * IT; ++k) {
-          const int j = threadIdx.x + k * threads, u = j % units, at = j / units;
-          if (at >= at0 && at < at1) {
-            const Unit n = unit_of(p, u);
-            uint32_t w[4];
-#pragma unroll
-            for (int m = 0; m < 4; ++m) w[m] = to_e4m3x4(x[k][4 * m] * inv, x[k][4 * m + 1] * inv, x[k][4 * m + 2] * inv, x[k][4 * m + 3] * inv);
-            *(u32x2*)(base + k_at(p.dim, at, n.d0)) = u32x2{w[0], w[1]};
-            *(u32x2*)(base + k_at(p.dim, at, n.d1)) = u32x2{w[2], w[3]};
-          }
-        }
+        const float before_s = p.ks[ph], most = take(part0, h);
+        put(part0, p.kp + ph * head_bytes, scaled(h, most, before_s));
       }
       return;
     }
-    for (int h = h0; h < h1; ++h) {
-      const long ph = (long)page * p.kv_heads + h;
-      uint8_t* base = p.vp + ph * ((long)p.dim << p.t.page_shift);
-      const float before_s = p.vs[ph];
-      float most = 0.f;
-      u32x4 raw[IT][4];
+    float most[kHeads] = {}, inv[kHeads];
+    for (int part = part0; part <= part1; ++part) {
+      angles(part);
 #pragma unroll
-      for (int k = 0; k < IT; ++k) {
-        const int j = threadIdx.x + k * threads, d0 = (j & 7) * 8 + (j / (2 * P)) * 64, quad = j / 8 % (P / 4);
+      for (int i = 0; i < kHeads; ++i)
+        if (h0 + i < h1) most[i] = fmaxf(most[i], take(part, h0 + i));
+    }
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          const int at = 4 * quad + m;
-          raw[k][m] = u32x4{0, 0, 0, 0};
-          if (at >= at0 && at < at1) raw[k][m] = ld16(p.v + (long)(row0 + at) * p.v_tok + (long)h * p.v_head + d0);
+    for (int i = 0; i < kHeads; ++i)
+      if (h0 + i < h1) inv[i] = scaled(h0 + i, most[i], p.ks[(long)page * p.kv_heads + h0 + i]);
+    for (int part = part0; part <= part1; ++part) {
+      angles(part);
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i)
+        if (h0 + i < h1) {
+          take(part, h0 + i);
+          put(part, p.kp + ((long)page * p.kv_heads + h0 + i) * head_bytes, inv[i]);
         }
+    }
+    return;
+  }
+  u32x4 raw[IT][4];
+  auto d_of = [&](int j) { return (j & 7) * 8 + j / (2 * part_tokens) * 64; };
+  auto at_of = [&](int part, int j) { return part * part_tokens + 4 * (j / 8 % (part_tokens / 4)); };
+  auto take = [&](int part, int h) {
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+      const int j = threadIdx.x + k * threads;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const int at = at_of(part, j) + m;
+        raw[k][m] = u32x4{0, 0, 0, 0};
+        if (at >= at0 && at < at1) raw[k][m] = ld16(p.v + (long)(row0 + at) * p.v_tok + (long)h * p.v_head + d_of(j));
       }
+    }
+    float most = 0.f;
 #pragma unroll
-      for (int k = 0; k < IT; ++k)
+    for (int k = 0; k < IT; ++k)
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          float x[8];
-          unpack8<T>(raw[k][m], x);
+      for (int m = 0; m < 4; ++m) {
+        float x[8];
+        unpack8<T>(raw[k][m], x);
 #pragma unroll
-          for (int d = 0; d < 8; ++d) most = fmaxf(most, finite_abs(x[d]));
-        }
-      __syncthreads();  // (red)
-      const float inv = exp2i(-page_exponent(p, block_most(most, red), base, p.vs + ph, before_s, at0, true));
-#pragma unroll
-      for (int k = 0; k < IT; ++k) {
-        const int j = threadIdx.x + k * threads, d0 = (j & 7) * 8 + (j / (2 * P)) * 64, quad = j / 8 % (P / 4);
-        const int before = at0 - 4 * quad, behind = 4 * quad + 4 - at1;  // places of the four that stay as they are
-        if (before >= 4 || behind >= 4) continue;
-        float x[4][8];
-#pragma unroll
-        for (int m = 0; m < 4; ++m) unpack8<T>(raw[k][m], x[m]);
-        const uint32_t keep = (before > 0 ? (1u << (8 * before)) - 1u : 0u) | (behind > 0 ? ~(0xffffffffu >> (8 * behind)) : 0u);
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          uint32_t* to = (uint32_t*)(base + v_at(p.dim, 4 * quad, d0 + d));
-          uint32_t w = to_e4m3x4(x[0][d] * inv, x[1][d] * inv, x[2][d] * inv, x[3][d] * inv);
-          if (keep) w = (w & ~keep) | (*to & keep);
-          *to = w;
-        }
+        for (int d = 0; d < 8; ++d) most = fmaxf(most, finite_abs(x[d]));
       }
+    return most;
+  };
+  auto put = [&](int part, uint8_t* base, float inv) {
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+      const int j = threadIdx.x + k * threads, at = at_of(part, j);
+      const int before = at0 - at, behind = at + 4 - at1;  // places of the four that stay as they are
+      if (before >= 4 || behind >= 4) continue;
+      float x[4][8];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) unpack8<T>(raw[k][m], x[m]);
+      const uint32_t keep = (before > 0 ? (1u << (8 * before)) - 1u : 0u) | (behind > 0 ? ~(0xffffffffu >> (8 * behind)) : 0u);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        uint32_t* to = (uint32_t*)(base + v_at(p.dim, at, d_of(j) + d));
+        uint32_t w = to_e4m3x4(x[0][d] * inv, x[1][d] * inv, x[2][d] * inv, x[3][d] * inv);
+        if (keep) w = (w & ~keep) | (*to & keep);
+        *to = w;
+      }
+    }
+  };
+  for (int h = h0; h < h1; ++h) {
+    const long ph = (long)page * p.kv_heads + h;
+    uint8_t* base = p.vp + ph * head_bytes;
+    const float before_s = p.vs[ph];
+    float most = take(part0, h);
+    for (int part = part0 + 1; part <= part1; ++part) most = fmaxf(most, take(part, h));
+    __syncthreads();  // (red)
+    const float inv = exp2i(-page_exponent(p, block_most(most, red), base, p.vs + ph, before_s, at0, true));
+    put(part1, base, inv);  // (the one that was read last)
+    for (int part = part0; part < part1; ++part) {
+      take(part, h);
+      put(part, base, inv);
     }
   }
 }
@@ -459,8 +510,8 @@ extern "C" int mui_paged_append(mui_stream_t stream, const mui_paged_append_args
       hipLaunchKernelGGL((append_step_kernel<BF16>), dim3((unsigned)blocks), dim3(256), 0, s, p);
     return launch_status();
   }
-  // 32 values a thread, of the larger pages 64 and 128
-  const int values = a.page_tokens * a.head_dim / 32, threads = values < 512 ? values : 512;
+  const bool full = a.n_rows > (long)a.n_requests * a.page_tokens;  // pages are filled, as a rule
+  const int values = a.page_tokens * a.head_dim / 32, threads = values < 512 ? values : full && values == 1024 ? 1024 : 512;
   const long rows_per = threads / units;
   const long q_blocks = a.q ? (a.n_rows + rows_per - 1) / rows_per * ((a.n_q_heads + kQueryHeads - 1) / kQueryHeads) : 0;
   const long pages = (long)a.n_rows / a.page_tokens + 2 * (long)a.n_requests;  // that new tokens can lie in
@@ -471,11 +522,10 @@ extern "C" int mui_paged_append(mui_stream_t stream, const mui_paged_append_args
   if (blocks > 0x7fffffffL) return MUI_ERR_UNSUPPORTED;
   p.q_blocks = (int)q_blocks;
   const dim3 grid((unsigned)blocks), block(threads);
-#define MUI_APPEND_GO(TT)                                                                             \
-  do {                                                                                                \
-    if (values <= 512) hipLaunchKernelGGL((append_rows_kernel<TT, 1>), grid, block, 0, s, p);         \
-    else if (values == 1024) hipLaunchKernelGGL((append_rows_kernel<TT, 2>), grid, block, 0, s, p);   \
-    else hipLaunchKernelGGL((append_rows_kernel<TT, 4>), grid, block, 0, s, p);                       \
+#define MUI_APPEND_GO(TT)                                                                                     \
+  do {                                                                                                        \
+    if (values <= 1024 || !full) hipLaunchKernelGGL((append_rows_kernel<TT, 1>), grid, block, 0, s, p);       \
+    else hipLaunchKernelGGL((append_rows_kernel<TT, 4>), grid, block, 0, s, p);                               \
   } while (0)
   if (a.dtype == MUI_DTYPE_F16) MUI_APPEND_GO(F16); else MUI_APPEND_GO(BF16);
   return launch_status();
