@@ -474,3 +474,17 @@ def test_captured_prompts_and_joined_results():
         assert torch.equal(out[0], again[0]) and torch.equal(out[1], again[1]), n
         want, bound = attention(cache, q[:2].cpu(), table.cpu(), n, [1, 1], dim ** -0.5)
         check(out[1], want, bound, str(n))
+
+
+@pytest.mark.parametrize("dtype,dim", [(F16, 128), (BF16, 64)])
+def test_longer_prompts_of_many_requests(dtype, dim):
+    """More than 64 requests on the kernel for prompts, and more than are dealt out, most of them with one new token."""
+    g = torch.Generator().manual_seed(5)
+    new = torch.randint(20, 60, (80,), generator=g).tolist()
+    new[3], new[63], new[64], new[79] = 0, 1, 120, 0
+    lengths = [n + int(torch.randint(0, 300, (1,), generator=g)) for n in new]
+    run_attention(dtype, dim, 64, lengths, new, 8, 1)
+    new = [1] * 1100
+    new[5], new[600], new[700], new[1099] = 40, 0, 33, 17
+    lengths = [n + i % 7 for i, n in enumerate(new)]
+    run_attention(dtype, dim, 64, lengths, new, 8, 1, max_tokens=40)
