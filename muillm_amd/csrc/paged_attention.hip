@@ -1077,7 +1077,9 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
   // 12.3 / 15.6; 128 dimensions, one of 1400 17.2 / 16.0, 30 20.9 / 23.6, one of 2000 20.0 / 14.4, 30 26.3 / 31.6; 256 dimensions, 30 of 800 25.1 / 28.0, 8 of 1400 27.6 / 23.6.
   const bool unit = !sparse && (tiles <= (head_dim == 256 ? 16 : 24) || n_requests > kDealtRequests);
   const bool dealt = !unit && n_requests <= kDealtRequests && (long)n_requests * each(16) <= 0x3fffffffL / tiles / n_kv_heads;
-  const bool prompt = !(unit || dealt) || (2 * all(16) - 3 * all(wide)) * n_kv_heads >= (12000 + tiles - 1) / tiles;
+  // (more than two rounds of units, of several a request, are begun and ended for nothing: 11 requests of up to 238 keys and 155 new tokens, 28 heads, 50 us, on the prompts' kernel 21)
+  const bool rounds = unit && each(16) > 1 && all(16) * n_kv_heads > 512;
+  const bool prompt = !(unit || dealt) || rounds || (2 * all(16) - 3 * all(wide)) * n_kv_heads >= (12000 + tiles - 1) / tiles;
   r.block_cols = prompt ? wide : 16;
   r.col_tiles = (int)each(r.block_cols);
   const long units = n_kv_heads * all(r.block_cols);
@@ -1085,12 +1087,18 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
   r.splits = 1;
   r.split_tiles = (int)tiles;
   if (prompt) {
-    // Keys divided among the workgroups that the card has room for at once, 8 tiles each at least. us with room for 256 / 512 / 1024: 100 new tokens of 4 requests of 8000 keys 104 / 84 / 93,
-    // 64 of one of 30000 66 / 65 / 89; tiles 8 / 16: 64 of one of 8000 35 / 39, 128 of two of 2000 30 / 37. The new tokens' own
-    // tiles count half, since as many are not seen: 1000 of one of 1000 takes 42 in two parts, 30 in one.
-    long splits = (head_dim == 256 ? 256 : 512) / units;
-    if (splits > (tiles - max_tokens / 128) / 8) splits = (tiles - max_tokens / 128) / 8;
-    if (splits < 1) splits = 1;
+    // Keys divided among the workgroups that the card has room for at once, 8 tiles each at least, where that ends earlier: a workgroup takes 1.4 us a tile, two on a CU 2.2 (256 dimensions,
+    // one on a CU: 2.5), joining 10. us undivided / divided: 1000 tokens of one request 30 / 42 (two parts), 100 of 4 requests of 8000 keys 104 (two) / 82 (four), two of 1477, one KV head,
+    // 51 / 43 (two); 256 dimensions, 500 behind 1000 49 / 67 (more than there is room for), 64 behind 8000 59 / 45.
+    const long room = head_dim == 256 ? 256 : 512;
+    long splits = 1, least = 0;
+    for (long n = 1; n == 1 || (n <= tiles / 8 && n * units <= room); n += 1 + n / 16) {
+      const long ns = (head_dim == 256 ? 2500 : n * units <= 256 ? 1400 : 2200) * ((tiles + n - 1) / n) + (n > 1 ? 10000 : 0);
+      if (n == 1 || ns < least) {
+        least = ns;
+        splits = n;
+      }
+    }
     r.split_tiles = (int)((tiles + splits - 1) / splits);
     r.splits = (int)((tiles + r.split_tiles - 1) / r.split_tiles);
     r.scratch = r.splits > 1 ? (size_t)r.splits * n_rows * n_q_heads * (head_dim + 4) * 4 : 0;
