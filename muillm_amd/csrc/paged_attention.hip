@@ -1077,7 +1077,7 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
   // 12.3 / 15.6; 128 dimensions, one of 1400 17.2 / 16.0, 30 20.9 / 23.6, one of 2000 20.0 / 14.4, 30 26.3 / 31.6; 256 dimensions, 30 of 800 25.1 / 28.0, 8 of 1400 27.6 / 23.6.
   const bool unit = !sparse && (tiles <= (head_dim == 256 ? 16 : 24) || n_requests > kDealtRequests);
   const bool dealt = !unit && n_requests <= kDealtRequests && (long)n_requests * each(16) <= 0x3fffffffL / tiles / n_kv_heads;
-  // (more than two rounds of units, of several a request, are begun and ended for nothing: 11 requests of up to 238 keys and 155 new tokens, 28 heads, 50 us, on the prompts' kernel 21)
+  // (more than two rounds of units, of several a request, are begun and ended for nothing: 11 requests of up to 238 keys and 155 new tokens, 28 heads, 50 us, on the prompts' kernel 19)
   const bool rounds = unit && each(16) > 1 && all(16) * n_kv_heads > 512;
   const bool prompt = !(unit || dealt) || rounds || (2 * all(16) - 3 * all(wide)) * n_kv_heads >= (12000 + tiles - 1) / tiles;
   r.block_cols = prompt ? wide : 16;
