@@ -1,10 +1,10 @@
 // What the kernels over a paged e4m3 cache share: its layout, its scales, the 8-bit conversions.
 //
 // A layer's cache has pages of P tokens (a multiple of 64). Of one page and KV head the keys are [P / 64][D / 64][64 tokens][64 dimensions]
-// and the values [P / 64][D][64], whose 64 bytes are the tokens 16 t + 4 g + i in the order (g, t, i): what lane (row, g) of a 16 x 16 x 128 matrix
-// instruction holds of either is then 16 bytes in a row, a wave's load is 1 KB in a row, and the probabilities of 64 keys, which the score
-// products leave in the order (t, i) at lane group g, are the other operand as they are. Scales are powers of two, so that appending a louder token to
-// a page moves the exponents of its codes (only what falls among e4m3's subnormals is rounded again), and the matrix cores take them as block exponents.
+// and the values [P / 64][D][64], whose 64 bytes are the tokens 16 t + 4 g + i in the order (g, t, i): what lane (row, g) holds of two
+// 16 x 16 x 32 matrix instructions' operands is then 16 bytes in a row, a wave's load is 1 KB in a row, and the probabilities of 64 keys, which the score
+// products leave in the order (t, i) at lane group g, are the other operands as they are. Scales are powers of two, so that appending a louder token to
+// a page moves the exponents of its codes (only what falls among e4m3's subnormals is rounded again), and what is multiplied by one loses nothing.
 #pragma once
 
 #include "hybrid.cuh"

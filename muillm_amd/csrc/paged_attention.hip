@@ -1,9 +1,9 @@
 // Attention over a paged e4m3 cache (paged.cuh has its layout).
 //
-// The matrix cores take the codes as they lie in memory: v_mfma_scale_f32_16x16x128_f8f6f4, whose block exponents carry the pages' scales. What
-// meets them is split into pieces of e4m3 so that nothing is lost by it: a query into two (bf16: 8 bits are two pieces of 4) or three (fp16), each 2^5 below
-// the one before; a probability into two (fp16: three), of 8 (12) bits together, relative to the largest of its query's 64 in the tile (2^-18 of it at least), which goes
-// with the product as its block exponent -- so a tile whose keys weigh little is as exact as one whose weigh much, however long the cache.
+// Codes are widened to 16 bits, which hold them whole, and meet the queries in the queries' own type: scores are sums of exact products in 32 bits. (The matrix cores' 8-bit
+// instructions take codes as they lie, but keep 13 bits below the largest of a lane's products: keys that have a channel in common, as trained models' do, lost all that tells
+// them apart.) Probabilities meet the values in fp16: relative to the largest of a query's 64 in a tile (single tokens, two pieces of 11 bits each) or to a running reference
+// (prompts: one piece for bf16 outputs, whose own rounding is 8 times as coarse, two for fp16).
 // Sums and the running maximum are 32 bits; the maximum is rounded up to a whole power of two, so moving to a new one is exact.
 //
 // Score products are K Q^T (rows keys, columns queries), value products V^T P^T: scores leave the first as the second wants them, in registers.
@@ -60,15 +60,31 @@ __device__ __forceinline__ TileRange tile_range(const PagedAttnParams& p, long f
 
 __device__ __forceinline__ i32x8 pair8(u32x4 a, u32x4 b) { return i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w}; }
 
-__device__ __forceinline__ f32x4 mfma_e4m3(i32x8 a, i32x8 b, f32x4 c, int scale_a, int scale_b) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, scale_a, 0, scale_b);
+// (counts; not for sums: within an instruction the matrix cores keep 13 bits below the largest of a lane's products)
+__device__ __forceinline__ f32x4 mfma_e4m3(i32x8 a, i32x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 127, 0, 127);
 }
 
-// 16 columns of queries as the score products want them: lane (column l % 16, g = l / 16) has of every 64 dimensions the 16 from 16 g on.
-template <int DC, int PIECES>
+// Two of four codes in 16 bits, which hold every e4m3 number.
+template <typename T>
+__device__ __forceinline__ uint32_t widen2(uint32_t w, bool high) {
+  if constexpr (T::kDtype == MUI_DTYPE_F16)
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true)) : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+  else
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true)) : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
+}
+template <typename T>
+__device__ __forceinline__ u32x4 widen8(uint32_t a, uint32_t b) { return u32x4{widen2<T>(a, false), widen2<T>(a, true), widen2<T>(b, false), widen2<T>(b, true)}; }
+
+// the same in fp16 times a power of two
+__device__ __forceinline__ uint32_t scaled2(uint32_t w, float s, bool high) {
+  return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true)) : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false));
+}
+
+// 16 columns of queries as the score products want them: lane (column l % 16, g = l / 16) has of every 64 dimensions the 16 from 16 g on, 8 for each of two products.
+template <int DC>
 struct QueryTile {
-  static constexpr int M = (DC + 1) / 2;
-  i32x8 piece[PIECES][M];
+  u32x4 v[DC][2];
   float unit;  // what the products are multiplied by, the score scale included
 };
 template <int DC>
@@ -83,51 +99,42 @@ __device__ __forceinline__ QueryRow<DC> request_queries(const uint16_t* row, int
   }
   return r;
 }
-template <typename T, int DC, int PIECES>
-__device__ __forceinline__ void take_queries(QueryTile<DC, PIECES>& t, const QueryRow<DC>& row, bool there, float score_scale, int g) {
-  float x[DC][16];
-  float most = 0.f;
+// fp16 queries go in as they are; of bf16 ones the row's largest is brought below 2^8 by a power of two, so that no sum of their products with codes overflows
+template <typename T, int DC>
+__device__ __forceinline__ void take_queries(QueryTile<DC>& t, const QueryRow<DC>& row, bool there, float score_scale) {
+  t.unit = score_scale;
+  const u32x4 zero = {0, 0, 0, 0};
 #pragma unroll
-  for (int c = 0; c < DC; ++c) {
-    const u32x4 zero = {0, 0, 0, 0};
-    float a[8], b[8];
-    unpack8<T>(there ? row.v[c][0] : zero, a);
-    unpack8<T>(there ? row.v[c][1] : zero, b);
+  for (int c = 0; c < DC; ++c)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[c][i] = a[i];
-      x[c][8 + i] = b[i];
-      most = fmaxf(most, fmaxf(fabsf(a[i]), fabsf(b[i])));
-    }
-  }
-  most = rows_max(most);
-  int e = (int)((__float_as_uint(most) >> 23) & 0xff) - 126 - 8;  // |x| 2^-e < 2^8
-  e = e < -110 ? -110 : (e > 119 ? 119 : e);
-  t.unit = exp2i(e) * score_scale;
-  const float inv = exp2i(-e);
-  uint32_t w[PIECES][2 * QueryTile<DC, PIECES>::M][4];
+    for (int j = 0; j < 2; ++j) t.v[c][j] = there ? row.v[c][j] : zero;
+  if constexpr (T::kDtype == MUI_DTYPE_BF16) {
+    float most = 0.f;
 #pragma unroll
-  for (int c = 0; c < 2 * QueryTile<DC, PIECES>::M; ++c) {
+    for (int c = 0; c < DC; ++c)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float r[4];
+      for (int j = 0; j < 2; ++j) {
+        float x[8];
+        unpack8<T>(t.v[c][j], x);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = c < DC ? x[c < DC ? c : 0][4 * j + i] * inv : 0.f;
-#pragma unroll
-      for (int s = 0; s < PIECES; ++s) {
-        const uint32_t v = to_e4m3x4(r[0], r[1], r[2], r[3]);
-        w[s][c][j] = v;
-        const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)v, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)v, true);
-        r[0] = (r[0] - a[0]) * 32.f; r[1] = (r[1] - a[1]) * 32.f; r[2] = (r[2] - b[0]) * 32.f; r[3] = (r[3] - b[1]) * 32.f;
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
       }
-    }
+    most = rows_max(most);
+    int e = (int)((__float_as_uint(most) >> 23) & 0xff) - 126 - 8;  // |x| 2^-e < 2^8
+    e = e < -110 ? -110 : (e > 119 ? 119 : e);
+    t.unit = exp2i(e) * score_scale;
+    const float inv = exp2i(-e);
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float x[8];
+        unpack8<T>(t.v[c][j], x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= inv;
+        t.v[c][j] = pack8<T>(x);
+      }
   }
-#pragma unroll
-  for (int s = 0; s < PIECES; ++s)
-#pragma unroll
-    for (int m = 0; m < QueryTile<DC, PIECES>::M; ++m)
-      t.piece[s][m] = pair8(u32x4{w[s][2 * m][0], w[s][2 * m][1], w[s][2 * m][2], w[s][2 * m][3]},
-                            u32x4{w[s][2 * m + 1][0], w[s][2 * m + 1][1], w[s][2 * m + 1][2], w[s][2 * m + 1][3]});
 }
 
 // One tile of 64 keys. A chunk of 1 KB is one operand of a wave: lane (row l % 16, g) has chunk g of the row's 64 bytes.
@@ -177,8 +184,9 @@ __device__ __forceinline__ void times_here(f32x4& x, float f) {
 }
 
 // What a tile's score products are multiplied by. Not 0, which a query and keys of zeros would make it (2^-120 is a page's scale then): a hidden key's score is -inf. Nor more
-// than leaves the largest products finite.
-__device__ __forceinline__ float score_unit(float query, float keys) { return __builtin_amdgcn_fmed3f(query * keys, 0x1p-126f, 0x1p100f); }
+// than leaves the largest products finite (256 of 2^8 times 448, of fp16 2^16 times 448).
+template <typename T>
+__device__ __forceinline__ float score_unit(float query, float keys) { return __builtin_amdgcn_fmed3f(query * keys, 0x1p-126f, T::kDtype == MUI_DTYPE_F16 ? 0x1p94f : 0x1p100f); }
 
 // Scores so far from zero that what a fused product keeps and a maximum has rounded away counts in an exponential: they are rounded first.
 __device__ __forceinline__ bool is_far(float most) { return fabsf(most) >= 0x1p22f && most > kNoMax; }
@@ -199,20 +207,18 @@ struct Columns {
 
 // The tile's scores and values into the results of 16 columns. pos: the lane's column's position (-1: no column); first_key: key 0 of the tile;
 // whole: every column sees all 64 keys. `ks`, `vs`: the page's scales.
-template <int DC, int PIECES>
-__device__ __forceinline__ void attend_tile(Columns<DC>& c, const QueryTile<DC, PIECES>& q, const KvRegs<DC>& kv, float ks, float vs, bool whole, long first_key, long pos,
+template <typename T, int DC>
+__device__ __forceinline__ void attend_tile(Columns<DC>& c, const QueryTile<DC>& q, const KvRegs<DC>& kv, float ks, float vs, bool whole, long first_key, long pos,
                                             long length, int window, int keep, int g) {
-  constexpr int M = (DC + 1) / 2;
-  const u32x4 zero = {0, 0, 0, 0};
   f32x4 s[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      const i32x8 kk = pair8(kv.kr[8 * m + i], 2 * m + 1 < DC ? kv.kr[2 * m + 1 < DC ? 8 * m + 4 + i : 0] : zero);
-#pragma unroll
-      for (int j = 0; j < PIECES; ++j) s[i] = mfma_e4m3(kk, q.piece[j][m], s[i], 127, 127 - 5 * j);
+    for (int cc = 0; cc < DC; ++cc) {
+      const u32x4 k = kv.kr[4 * cc + i];
+      s[i] = mfma16x16x32<T>(widen8<T>(k.x, k.y), q.v[cc][0], s[i]);
+      s[i] = mfma16x16x32<T>(widen8<T>(k.z, k.w), q.v[cc][1], s[i]);
     }
   }
   uint32_t seen = 0xffffu;
@@ -223,7 +229,7 @@ __device__ __forceinline__ void attend_tile(Columns<DC>& c, const QueryTile<DC, 
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[i][r] = seen >> (4 * i + r) & 1u ? s[i][r] : -INFINITY;
   }
-  float unit = score_unit(q.unit, ks);
+  float unit = score_unit<T>(q.unit, ks);
   float most = s[0][0];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -243,31 +249,32 @@ __device__ __forceinline__ void attend_tile(Columns<DC>& c, const QueryTile<DC, 
 #pragma unroll
     for (int i = 0; i < 4 * DC; ++i) c.o[i] *= f;
   }
-  // probabilities of the tile, its largest in (2^7, 2^8]
-  const float base = fabsf(mt) < 0x1p24f ? mt - 8.f : mt;  // (beyond, the difference would be rounded)
-  i32x8 pp, rest;  // rest: fp16's third pieces, each 2^5 below what it adds to; the same values of the cache twice as in pp, the second time times zero
+  // probabilities of the tile, its largest in (2^13, 2^14]
+  const float base = fabsf(mt) < 0x1p24f ? mt - 14.f : mt;  // (beyond, the difference would be rounded)
+  u32x4 hi[2], lo[2];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float e[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], unit, -base));
-    const uint32_t hi = to_e4m3x4(e[0], e[1], e[2], e[3]);
-    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true);
-    pp[i] = (int)hi;
-    const float d[4] = {e[0] - a[0], e[1] - a[1], e[2] - b[0], e[3] - b[1]};
-    const uint32_t lo = to_e4m3x4(d[0], d[1], d[2], d[3]);
-    pp[4 + i] = (int)lo;
-    if constexpr (PIECES == 3) {
-      const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, false), y = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, true);
-      rest[i] = (int)to_e4m3x4(32.f * (d[0] - x[0]), 32.f * (d[1] - x[1]), 32.f * (d[2] - y[0]), 32.f * (d[3] - y[1]));
-      rest[4 + i] = 0;
+#pragma unroll
+    for (int r = 0; r < 4; r += 2) {
+      const uint32_t w = F16::pack2(e[r], e[r + 1]);
+      hi[i >> 1][2 * (i & 1) + r / 2] = w;
+      lo[i >> 1][2 * (i & 1) + r / 2] = F16::pack2(e[r] - F16::lo(w), e[r + 1] - F16::hi(w));
     }
   }
-  const int sb = 127 + (int)fmaxf(base - c.m, -127.f), sa = 127 + scale_exponent(vs);
-  constexpr int kOnes = 0x38383838;
-  const i32x8 ones = {kOnes, kOnes, kOnes, kOnes, kOnes, kOnes, kOnes, kOnes};
-  c.l = mfma_e4m3(ones, pp, c.l, 127, sb);
-  if constexpr (PIECES == 3) c.l = mfma_e4m3(ones, rest, c.l, 122, sb);
+  const int down = (int)fmaxf(base - c.m, -300.f);
+  const float f = __builtin_amdgcn_ldexpf(vs, down);
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  const u32x4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+  auto product = [&](u32x4 v0, u32x4 v1) {
+    f32x4 t = mfma16x16x32<F16>(v0, lo[0], zero);
+    t = mfma16x16x32<F16>(v1, lo[1], t);
+    t = mfma16x16x32<F16>(v0, hi[0], t);
+    return mfma16x16x32<F16>(v1, hi[1], t);
+  };
+  c.l += product(ones, ones) * __builtin_amdgcn_ldexpf(1.f, down);
   // Where part of the tile is hidden, what stands there may be anything, and 0 * NaN is NaN.
   bool nan = false;
   if (!whole) {
@@ -282,22 +289,18 @@ __device__ __forceinline__ void attend_tile(Columns<DC>& c, const QueryTile<DC, 
   }
   if (!nan) {
 #pragma unroll
-    for (int i = 0; i < 4 * DC; ++i) {
-      const i32x8 vv = pair8(kv.vr[i], kv.vr[i]);
-      c.o[i] = mfma_e4m3(vv, pp, c.o[i], sa, sb);
-      if constexpr (PIECES == 3) c.o[i] = mfma_e4m3(vv, rest, c.o[i], sa - 5, sb);
-    }
+    for (int i = 0; i < 4 * DC; ++i) c.o[i] += product(widen8<F16>(kv.vr[i].x, kv.vr[i].y), widen8<F16>(kv.vr[i].z, kv.vr[i].w)) * f;
     return;
   }
   // A NaN code counts as zero, and a column that sees it gets a NaN.
-  i32x8 mine;
+  const u32x4 none = {0, 0, 0, 0};
+  u32x4 mine;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t w = 0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) w |= seen >> (4 * i + r) & 1u ? 0x38u << (8 * r) : 0u;
-    mine[i] = (int)w;
-    mine[4 + i] = 0;
+    mine[i] = w;
   }
 #pragma unroll
   for (int i = 0; i < 4 * DC; ++i) {
@@ -309,9 +312,8 @@ __device__ __forceinline__ void attend_tile(Columns<DC>& c, const QueryTile<DC, 
       v[j] &= ~x[j];
       x[j] &= 0x38383838u;
     }
-    c.o[i] = mfma_e4m3(pair8(v, v), pp, c.o[i], sa, sb);
-    if constexpr (PIECES == 3) c.o[i] = mfma_e4m3(pair8(v, v), rest, c.o[i], sa - 5, sb);
-    const f32x4 sees = mfma_e4m3(pair8(x, zero), mine, f32x4{0.f, 0.f, 0.f, 0.f}, 127, 127);
+    c.o[i] += product(widen8<F16>(v.x, v.y), widen8<F16>(v.z, v.w)) * f;
+    const f32x4 sees = mfma_e4m3(pair8(x, none), pair8(mine, none), zero);
 #pragma unroll
     for (int r = 0; r < 4; ++r) c.o[i][r] = sees[r] > 0.f ? __builtin_nanf("") : c.o[i][r];
   }
@@ -371,7 +373,7 @@ __device__ __forceinline__ PagedSpan span_of_lane(const PagedSpan& s, int l) {
 // while one is worked on as well their registers do not suffice (64 requests of 4096 to 16384 tokens 204 instead of 187 us).
 // The cache's bytes bound it where there are many: those 64 requests, 8 KV heads of 128 dimensions (1.17 GB), 187 us, 6.2 TB/s; 32 requests of 200 to 4096 (90 MB) 29.6. With few it is the loads that
 // wait for one another (length, page, keys and values, again for each tile of a wave): 700 keys 9.4 us.
-template <typename T, int DC, int PIECES, int W>
+template <typename T, int DC, int W>
 __global__ void __launch_bounds__(64 * W, DC == 4 ? W / 4 : 2) paged_columns_kernel(const PagedAttnParams p) {
   constexpr int D = DC * 64, kThreads = 64 * W;
   __shared__ float so[W][16][D + 4];
@@ -465,13 +467,13 @@ __global__ void __launch_bounds__(64 * W, DC == 4 ? W / 4 : 2) paged_columns_ker
     int page = page_of(tile0 + wave);
     TilePlace at = tile_place(p, page, range.at(tile0 + wave), h);
     if (page >= 0) t.load(p.kp + at.at * (64 * D), p.vp + at.at * (64 * D), lane);
-    QueryTile<DC, PIECES> q;
-    take_queries<T, DC, PIECES>(q, query, there, p.scale, g);
+    QueryTile<DC> q;
+    take_queries<T, DC>(q, query, there, p.scale);
     for (int i = tile0 + wave; i < end; i += W) {
       const int page1 = page_of(i + W);
       if (page >= 0) {
         const long k0 = 64L * range.at(i);
-        attend_tile<DC, PIECES>(c, q, t, at.ks, at.vs, sees_whole(p, k0, cb.pos0, cb.pos1, sp.length), k0, pos, sp.length, p.window, p.keep, g);
+        attend_tile<T, DC>(c, q, t, at.ks, at.vs, sees_whole(p, k0, cb.pos0, cb.pos1, sp.length), k0, pos, sp.length, p.window, p.keep, g);
       }
       page = page1;
       at = tile_place(p, page, range.at(i + W), h);
@@ -577,25 +579,10 @@ __global__ void __launch_bounds__(256) paged_join_units_kernel(const PagedAttnPa
 // ---------------------------------------------------------------------------------------
 // prompts
 // ---------------------------------------------------------------------------------------
-// Here the vector ALU is what counts beside the matrix cores (an exponential per key and query), so probabilities go into the value products whole, in the queries'
-// type, and values are converted to it once for the workgroup: 16 conversions a thread and tile in place of 100 instructions of splitting and of operands put together.
-// A probability is taken relative to a power of two that moves only if a maximum passes it by kRoom: for fp16 so that the largest are 2^7 to 2^15, what is 2^-21 of
-// the largest still has all its bits and what is 2^-31 of it some; bf16 has the exponents for anything.
-template <typename T> struct PromptType;
-template <> struct PromptType<BF16> {
-  static constexpr float kBias = 0.f, kRoom = 8.f;
-  static constexpr uint32_t kOne = 0x3f80u;
-  static __device__ __forceinline__ uint32_t codes(uint32_t w, float s, bool high) {
-    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true)) : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
-  }
-};
-template <> struct PromptType<F16> {
-  static constexpr float kBias = 7.f, kRoom = 8.f;
-  static constexpr uint32_t kOne = 0x3c00u;
-  static __device__ __forceinline__ uint32_t codes(uint32_t w, float s, bool high) {
-    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true)) : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false));
-  }
-};
+// Codes are widened once for the workgroup, on their way to LDS: keys to the queries' type, values to fp16 (keys widened by every
+// wave behind LDS, 8 KB less of it to read per tile, took 6 % longer). A probability is taken relative to a power of two that moves only if a maximum passes it by kRoom, so that the largest are 2^7 to
+// 2^15; what is 2^-21 of the largest still has all its bits in one piece.
+constexpr float kBias = 7.f, kRoom = 8.f;
 
 template <int DC>
 struct PromptColumns {
@@ -604,43 +591,41 @@ struct PromptColumns {
   float m, to;  // what probabilities are relative to: 2^m; kBias - m
 };
 
-// a tile in LDS as a wave's lanes have its operands: keys as codes (chunk i: 16 keys and 64 dimensions), values in the queries' type (16 dimensions, 32 keys)
+// a tile in LDS as a wave's lanes have its operands: keys in the queries' type (chunk i: 16 keys and 64 dimensions, in halves), values in fp16 (16 dimensions, 32 keys)
 struct PromptTile {
   const u32x4* kp; const u32x4* vp;
-  __device__ __forceinline__ u32x4 k(int i) const { return kp[i * 64]; }
+  __device__ __forceinline__ u32x4 k(int i, int half) const { return kp[(2 * i + half) * 64]; }
   __device__ __forceinline__ u32x4 v(int i, int half) const { return vp[(2 * i + half) * 64]; }
 };
 
 // scores of a tile
-template <int DC, int PIECES, int NT>
-__device__ __forceinline__ void prompt_scores(f32x4 (&s)[NT][4], const QueryTile<DC, PIECES> (&q)[NT], const PromptTile& t) {
-  constexpr int M = (DC + 1) / 2;
-  const u32x4 zero = {0, 0, 0, 0};
+template <typename T, int DC, int NT>
+__device__ __forceinline__ void prompt_scores(f32x4 (&s)[NT][4], const QueryTile<DC> (&q)[NT], const PromptTile& t) {
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {  // (two chunks' products between one product and the next on its result)
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      i32x8 kk[2];
+    for (int c = 0; c < DC; ++c) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) kk[k] = pair8(t.k(8 * m + i + k), 2 * m + 1 < DC ? t.k(2 * m + 1 < DC ? 8 * m + 4 + i + k : 0) : zero);
+      for (int j = 0; j < 2; ++j) {
+        u32x4 kk[2];
 #pragma unroll
-      for (int j = 0; j < PIECES; ++j)
+        for (int x = 0; x < 2; ++x) kk[x] = t.k(4 * c + i + x, j);
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) s[n][i + k] = mfma_e4m3(kk[k], q[n].piece[j][m], m || j ? s[n][i + k] : f32x4{0.f, 0.f, 0.f, 0.f}, 127, 127 - 5 * j);
+          for (int n = 0; n < NT; ++n) s[n][i + x] = mfma16x16x32<T>(kk[x], q[n].v[c][j], c || j ? s[n][i + x] : f32x4{0.f, 0.f, 0.f, 0.f});
+      }
     }
   }
 }
 
 // The reference of the probabilities moves where the tile's largest score (of this lane's keys) passes it by kRoom.
-template <typename T, int DC, int NT>
+template <int DC, int NT>
 __device__ __forceinline__ void prompt_move(PromptColumns<DC> (&c)[NT], const float (&most)[NT], f32x4 (&s)[NT][4], float (&unit)[NT]) {
-  typedef PromptType<T> PT;
   bool moves = false, far = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    moves |= most[n] > c[n].m + PT::kRoom;
+    moves |= most[n] > c[n].m + kRoom;
     far |= is_far(most[n]);
   }
   if (__any(far)) {
@@ -655,10 +640,10 @@ __device__ __forceinline__ void prompt_move(PromptColumns<DC> (&c)[NT], const fl
     float f[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {  // (a column's four lanes move together)
-      const float mt = fmaxf(ceilf(rows_max(most[n])), kNoMax), to = mt > c[n].m + PT::kRoom ? mt : c[n].m;
+      const float mt = fmaxf(ceilf(rows_max(most[n])), kNoMax), to = mt > c[n].m + kRoom ? mt : c[n].m;
       f[n] = __builtin_amdgcn_exp2f(c[n].m - to);
       c[n].m = to;
-      c[n].to = fabsf(to) < 0x1p24f ? PT::kBias - to : -to;  // (beyond, the sum would be rounded)
+      c[n].to = fabsf(to) < 0x1p24f ? kBias - to : -to;  // (beyond, the sum would be rounded)
     }
     between_matrix();
 #pragma unroll
@@ -683,9 +668,9 @@ __device__ __forceinline__ void prompt_most(float (&most)[NT], const f32x4 (&s)[
   }
 }
 
-// probabilities of a tile: unit = what its scores are multiplied by
-template <typename T, int DC, int NT>
-__device__ __forceinline__ void prompt_exp(u32x4 (&pp)[NT][2], const f32x4 (&s)[NT][4], const PromptColumns<DC> (&c)[NT], const float (&unit)[NT]) {
+// probabilities of a tile, in `PIECES` pieces: unit = what its scores are multiplied by
+template <int DC, int PIECES, int NT>
+__device__ __forceinline__ void prompt_exp(u32x4 (&pp)[NT][PIECES][2], const f32x4 (&s)[NT][4], const PromptColumns<DC> (&c)[NT], const float (&unit)[NT]) {
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -693,26 +678,33 @@ __device__ __forceinline__ void prompt_exp(u32x4 (&pp)[NT][2], const f32x4 (&s)[
       float e[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[n][i][r], unit[n], c[n].to));
-      pp[n][i >> 1][2 * (i & 1)] = T::pack2(e[0], e[1]);
-      pp[n][i >> 1][2 * (i & 1) + 1] = T::pack2(e[2], e[3]);
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const uint32_t w = F16::pack2(e[r], e[r + 1]);
+        pp[n][0][i >> 1][2 * (i & 1) + r / 2] = w;
+        if constexpr (PIECES == 2) pp[n][1][i >> 1][2 * (i & 1) + r / 2] = F16::pack2(e[r] - F16::lo(w), e[r + 1] - F16::hi(w));
+      }
     }
 }
 
-template <typename T, int DC, int NT>
-__device__ __forceinline__ void prompt_values(PromptColumns<DC> (&c)[NT], const u32x4 (&pp)[NT][2], const PromptTile& t) {
-  constexpr uint32_t kOnes = PromptType<T>::kOne * 0x10001u;
-  const u32x4 ones = {kOnes, kOnes, kOnes, kOnes};
+template <int DC, int PIECES, int NT>
+__device__ __forceinline__ void prompt_values(PromptColumns<DC> (&c)[NT], const u32x4 (&pp)[NT][PIECES][2], const PromptTile& t) {
+  const u32x4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 #pragma unroll
   for (int half = 0; half < 2; ++half)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) c[n].l = mfma16x16x32<T>(ones, pp[n][half], c[n].l);
+    for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) c[n].l = mfma16x16x32<F16>(ones, pp[n][k][half], c[n].l);
 #pragma unroll
   for (int i = 0; i < 4 * DC; ++i)
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const u32x4 v = t.v(i, half);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) c[n].o[i] = mfma16x16x32<T>(v, pp[n][half], c[n].o[i]);
+      for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) c[n].o[i] = mfma16x16x32<F16>(v, pp[n][k][half], c[n].o[i]);
     }
 }
 
@@ -736,7 +728,7 @@ __device__ __forceinline__ void prompt_nans(PromptColumns<DC> (&c)[NT], const ui
         for (int r = 0; r < 4; ++r) w |= seen[n] >> (4 * k + r) & 1u ? 0x38u << (8 * r) : 0u;
         mine[k] = w;
       }
-      const f32x4 sees = mfma_e4m3(pair8(x, zero), pair8(mine, zero), f32x4{0.f, 0.f, 0.f, 0.f}, 127, 127);
+      const f32x4 sees = mfma_e4m3(pair8(x, zero), pair8(mine, zero), f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
       for (int r = 0; r < 4; ++r) c[n].o[i][r] = sees[r] > 0.f ? __builtin_nanf("") : c[n].o[i][r];
     }
@@ -800,15 +792,14 @@ __device__ __forceinline__ bool nth_block(const PagedAttnParams& p, int n, int& 
 }
 
 // A workgroup of four waves takes 64 NT columns of one KV head (16 NT a wave) and `split_tiles` tiles, which its waves share through LDS: two tiles' room, the
-// next one's keys on their way to LDS and its values to registers while the waves work on one, one barrier a tile. Two such workgroups on a CU (one of 256 dimensions).
-// 2048 tokens behind 6144, 32 query and 8 KV heads of 128 bf16 dimensions (240 GFLOP): 225 us, 1.07 PFLOP/s, 8-bit products of queries in two pieces and 16-bit ones of values; the matrix
-// instructions alone would take 117 us at the clock that the card keeps under them. Of the rest the tile's way through LDS is 59 us, exponentials 18, maxima 13, the barrier 9.
-// Eight waves that share a tile take 318, probabilities and values in 8 bits 340 us (100 vector instructions a tile more).
-template <typename T, int DC, int PIECES, int NT>
+// next ones on their way to registers while the waves work on one, one barrier a tile. Two such workgroups on a CU (one of 256 dimensions).
+// 2048 tokens behind 6144, 32 query and 8 KV heads of 128 bf16 dimensions (240 GFLOP): 255 us, 0.94 PFLOP/s. The matrix instructions alone (1088 cycles of a SIMD for a
+// wave's 32 columns and a tile) take half of that at the clock that the card keeps under them; the rest is the tile's way through LDS (32 KB for each wave), exponentials and maxima.
+template <typename T, int DC, int NT>
 __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const PagedAttnParams p) {
   constexpr int D = DC * 64, kCols = 64 * NT;
-  typedef PromptType<T> PT;
-  __shared__ u32x4 keys[2][64 * D / 16], values[2][64 * D / 8];
+  constexpr int kPieces = T::kDtype == MUI_DTYPE_F16 ? 2 : 1;
+  __shared__ u32x4 keys[2][64 * D / 8], values[2][64 * D / 8];
   __shared__ int nan_tile[2];  // number of the tile + 1 where its values hold a NaN (looked for, and taken out, where not every column sees all of it)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = blockIdx.x % p.kv_heads;  // (neighbours go to different XCDs: of eight heads each XCD has one, whose keys stay in its L2)
@@ -822,7 +813,7 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
   const int end = begin + p.split_tiles < n_tiles ? begin + p.split_tiles : n_tiles;
   const int g = lane >> 4;
   if (threadIdx.x < 2) nan_tile[threadIdx.x] = 0;
-  QueryTile<DC, PIECES> q[NT];
+  QueryTile<DC> q[NT];
   PromptColumns<DC> c[NT];
   int token[NT];  // of the request's new ones, the lane's columns'; -1: no column
   const int wave_col = cb.first + wave * (16 * NT);
@@ -835,7 +826,7 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
     const bool there = col < cb.end;
     const unsigned at = there ? col : cb.end - 1, tok = at / (unsigned)p.group, head = at - tok * p.group;
     token[n] = there ? (int)tok : -1;
-    take_queries<T, DC, PIECES>(q[n], request_queries<DC>(p.q + (long)(sp.row0 + (int)tok) * p.q_tok + (long)(h * p.group + (int)head) * p.q_head, g), there, p.scale, g);
+    take_queries<T, DC>(q[n], request_queries<DC>(p.q + (long)(sp.row0 + (int)tok) * p.q_tok + (long)(h * p.group + (int)head) * p.q_head, g), there, p.scale);
 #pragma unroll
     for (int i = 0; i < 4 * DC; ++i) c[n].o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     c[n].l = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -847,10 +838,16 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
   // a tile's page is loaded a tile before it is looked at: what follows would wait for it
   auto entry_of = [&](int i) { return i < end ? paged_entry(p.t, b, cb.range.at(i) >> per_page) : -1; };
   auto page_of = [&](int entry) { return uniform(page_of_entry(p.t, entry)); };
-  auto fetch_keys = [&](const TilePlace& at, int slot) {
+  u32x4 rawk[DC];
+  auto fetch_keys = [&](const TilePlace& at) {
+#pragma unroll
+    for (int i = 0; i < DC; ++i) rawk[i] = ld16(p.kp + at.at * (64 * D) + (wave * DC + i) * 1024 + lane_at);
+  };
+  auto put_keys = [&](int slot) {
 #pragma unroll
     for (int i = 0; i < DC; ++i)
-      load_lds16((const uint16_t*)(p.kp + at.at * (64 * D) + (wave * DC + i) * 1024 + lane_at), (uint16_t*)&keys[slot][(wave * DC + i) * 64]);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) keys[slot][((wave * DC + i) * 2 + half) * 64 + lane] = widen8<T>(rawk[i][2 * half], rawk[i][2 * half + 1]);
   };
   u32x4 raw[DC];
   auto fetch_values = [&](const TilePlace& at) {
@@ -865,8 +862,9 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
     const int t = cb.range.at(tile_no);
     return t < seen_end && (t >= seen_from || t < seen_kept);
   };
-  // fp16 holds a page's values times 2^(7 - loudest) of the loudest page so far: all codes exactly, unless a page is 2^22 times quieter than another
-  int loudest = -126;
+  // The sums of values are relative to 2^level, and fp16 holds a page's values times 2^(7 - level): all codes exactly down to 2^22 below the level, which follows louder pages at once and
+  // quieter ones where they would lose bits, but not further than 2^60 below the loudest (what has been added up fits 2^62 relative to that). It begins where 2^(level - 7) is still normal.
+  int level = -119, loudest = -119;
   auto put_values = [&](const TilePlace& at, int slot, int tile_no, auto whole) {
     if (!decltype(whole)::value && !all_seen(tile_no)) {
       uint32_t found = 0;
@@ -880,27 +878,28 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
         }
       if (__any(found != 0) && lane == 0) nan_tile[slot] = tile_no + 1;
     }
-    float s = at.vs;
-    if constexpr (T::kDtype == MUI_DTYPE_F16) {
-      const int e = scale_exponent(at.vs);
-      if (e > loudest) {
-        const float f = exp2i(loudest - e < -126 ? -126 : loudest - e);
+    const int e = scale_exponent(at.vs);
+    if (e > level || e < level - 22) {
+      loudest = e > loudest ? e : loudest;
+      const int least = loudest - 60 > -119 ? loudest - 60 : -119, to = e > least ? e : least;
+      if (to != level) {
+        const float f = exp2i(level - to < -126 ? -126 : level - to);
         between_matrix();
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 4 * DC; ++i) times_here(c[n].o[i], f);
         between_matrix();
-        loudest = e;
+        level = to;
       }
-      s = exp2i(e - loudest + 7 < -126 ? -126 : e - loudest + 7);
     }
+    const float s = exp2i(e - level + 7 < -126 ? -126 : e - level + 7);
 #pragma unroll
     for (int i = 0; i < DC; ++i)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint32_t a = raw[i][2 * half], d = raw[i][2 * half + 1];
-        values[slot][((wave * DC + i) * 2 + half) * 64 + lane] = u32x4{PT::codes(a, s, false), PT::codes(a, s, true), PT::codes(d, s, false), PT::codes(d, s, true)};
+        values[slot][((wave * DC + i) * 2 + half) * 64 + lane] = u32x4{scaled2(a, s, false), scaled2(a, s, true), scaled2(d, s, false), scaled2(d, s, true)};
       }
   };
   // Tile i's probabilities and value products go with tile i + 1's scores: while the vector ALU takes exponentials the matrix cores have products that wait for nothing.
@@ -911,17 +910,20 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
   float most[NT], unit[NT];
   __syncthreads();  // (nan_tile)
   if (page >= 0) {
-    fetch_keys(at, 0);
+    fetch_keys(at);
     fetch_values(at);
+    put_keys(0);
     put_values(at, 0, begin, std::false_type());
   }
-  wait_loads<0>();
   __syncthreads();
-  if (page1 >= 0) fetch_keys(at1, 1);
+  if (page1 >= 0) {
+    fetch_keys(at1);
+    put_keys(1);
+  }
   // scores that may be hidden: tile number, its place in LDS, whether it has a page
   auto masked_scores = [&](int tile_no, int slot, bool there) {
     const long k0 = 64L * cb.range.at(tile_no);
-    if (there && mine && k0 <= my_pos1) prompt_scores<DC, PIECES, NT>(s, q, PromptTile{&keys[slot][lane], nullptr});
+    if (there && mine && k0 <= my_pos1) prompt_scores<T, DC, NT>(s, q, PromptTile{&keys[slot][lane], nullptr});
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const uint32_t seen = there && mine ? seen_bits(k0, token[n] < 0 ? -1 : sp.start + token[n], sp.length, p.window, p.keep, g) : 0u;
@@ -940,34 +942,33 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
     prompt_most<NT>(most, s);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      unit[n] = score_unit(q[n].unit, at.ks);
+      unit[n] = score_unit<T>(q[n].unit, at.ks);
       most[n] *= unit[n];
     }
-    prompt_move<T, DC, NT>(c, most, s, unit);
+    prompt_move<DC, NT>(c, most, s, unit);
   }
   int i = begin;
   auto step = [&](auto whole) {
     constexpr bool kWhole = decltype(whole)::value;  // all columns see all of tiles i and i + 1
     const int slot = (i - begin) & 1;
-    wait_loads<0>();
     __syncthreads();  // tile i's values and tile i + 1's keys are there, for all; the other rooms' readers are done
     asm volatile("" : "+v"(entry2));  // (not looked at earlier: it would be waited for)
     const int page2 = page_of(entry2);
     entry2 = entry_of(i + 3);
     const TilePlace at2 = tile_place(p, page2, cb.range.at(i + 2), h);
-    if (page2 >= 0) fetch_keys(at2, slot);
+    if (page2 >= 0) fetch_keys(at2);
     if (kWhole || page1 >= 0) fetch_values(at1);
-    u32x4 pp[NT][2];
+    u32x4 pp[NT][kPieces][2];
     const PromptTile here = {nullptr, &values[slot][lane]}, ahead = {&keys[slot ^ 1][lane], nullptr};
-    prompt_exp<T, DC, NT>(pp, s, c, unit);
+    prompt_exp<DC, kPieces, NT>(pp, s, c, unit);
     if constexpr (kWhole) {
-      prompt_scores<DC, PIECES, NT>(s, q, ahead);
-      prompt_values<T, DC, NT>(c, pp, here);
+      prompt_scores<T, DC, NT>(s, q, ahead);
+      prompt_values<DC, kPieces, NT>(c, pp, here);
     } else {
       if (i + 1 < end) masked_scores(i + 1, slot ^ 1, page1 >= 0);
       const long k0 = 64L * cb.range.at(i);
       if (page >= 0 && mine && k0 <= my_pos1) {
-        prompt_values<T, DC, NT>(c, pp, here);
+        prompt_values<DC, kPieces, NT>(c, pp, here);
         if (nan_tile[slot] == i + 1) {
           uint32_t seen[NT];
 #pragma unroll
@@ -979,11 +980,12 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
     prompt_most<NT>(most, s);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      unit[n] = score_unit(q[n].unit, at1.ks);
+      unit[n] = score_unit<T>(q[n].unit, at1.ks);
       most[n] *= unit[n];
     }
     if (kWhole || page1 >= 0) put_values(at1, slot ^ 1, i + 1, whole);
-    if (kWhole || i + 1 < end) prompt_move<T, DC, NT>(c, most, s, unit);
+    if (page2 >= 0) put_keys(slot);
+    if (kWhole || i + 1 < end) prompt_move<DC, NT>(c, most, s, unit);
     at1 = at2;
     page = page1;
     page1 = page2;
@@ -995,24 +997,23 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
     while (whole_now()) step(std::true_type());
     while (i < end && !whole_now()) step(std::false_type());
   }
-  const float loud = T::kDtype == MUI_DTYPE_F16 ? exp2i(loudest - 7 < -126 ? -126 : loudest - 7) : 1.f;
+  const float loud = exp2i(level - 7);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int col = wave_col + 16 * n + (lane & 15);
     if (col >= cb.end) continue;
     const unsigned token = (unsigned)col / (unsigned)p.group;
     const long row = (long)(sp.row0 + (int)token) * p.heads + h * p.group + (col - (int)token * p.group);
-    const float sum = c[n].l[0];
+    const float sum = c[n].l[0], inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
     if (p.part) {
       float* part = p.part + ((long)blockIdx.y * p.t.n_rows * p.heads + row) * (D + 4);
 #pragma unroll
-      for (int i = 0; i < 4 * DC; ++i) *(f32x4*)(part + 16 * i + 4 * g) = c[n].o[i] * loud;
+      for (int i = 0; i < 4 * DC; ++i) *(f32x4*)(part + 16 * i + 4 * g) = c[n].o[i] * inv * loud;
       if (g == 0) { part[D] = -c[n].to; part[D + 1] = sum; }
     } else {
-      const float inv = sum > 0.f || sum != sum ? loud / sum : 0.f;
 #pragma unroll
       for (int i = 0; i < 4 * DC; ++i) {
-        const f32x4 o = c[n].o[i] * inv;
+        const f32x4 o = c[n].o[i] * inv * loud;
         *(u32x2*)(p.out + row * D + 16 * i + 4 * g) = u32x2{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])};
       }
     }
@@ -1041,8 +1042,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   for (int i = 0; i < splits; ++i) m = fmaxf(m, part[i * step + D]);
   float sum = 0.f, o[DC] = {};
   for (int i = 0; i < splits; ++i) {
-    const float f = __builtin_amdgcn_exp2f(part[i * step + D] - m);
-    sum += f * part[i * step + D + 1];
+    const float f = __builtin_amdgcn_exp2f(part[i * step + D] - m) * part[i * step + D + 1];
+    sum += f;
 #pragma unroll
     for (int j = 0; j < DC; ++j) o[j] += f * part[i * step + 64 * j + lane];
   }
@@ -1069,9 +1070,9 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
     return filled < most ? filled : most;
   };
   const int wide = head_dim == 256 ? 64 : 128;  // (256 dimensions: results of 32 columns a wave do not fit its registers)
-  // The kernel for single tokens takes 2 ns for a block of 16 columns and a tile, the one for prompts 4 for a block of 128, and 6 us more to begin with and to join. us, the one / the other,
-  // 32 heads, 8 KV heads, 128 dimensions: one request of 1000 keys and 32 new tokens 12 / 23; of 8000 and 16 27 / 28, 32 35 / 30; 16 requests of 1000 and 16 24 / 31, 32 45 / 38; of 8000
-  // and 4 58 / 92, 8 97 / 85, 32 283 / 101.
+  // The kernel for single tokens takes 2.2 ns for a block of 16 columns and a tile, the one for prompts 5 to 6 for a block of 128, and 6 us more to begin with and to join. us, the one / the
+  // other, 32 heads, 8 KV heads, 128 bf16 dimensions: one request of 1000 keys and 32 new tokens 12 / 26; of 8000 and 16 24 / 31, 32 33 / 32; 16 requests of 1000 and 16 23 / 34, 32 42 / 39;
+  // of 8000 and 4 54 / 92, 8 93 / 96 (fp16 93 / 114, 64 dimensions 41 / 74, 256 138 / 179), 32 281 / 119.
   const bool sparse = (long)n_requests * each(16) > 2 * all(16);  // a workgroup per unit would find most of them empty: those that begin and end take 8 ns each
   // A workgroup per unit needs no scan and no joining launch. us, a unit each / dealt out, 8 KV heads, requests of equal lengths, which suit it best: 64 dimensions, 8 requests of 1400 keys
   // 12.3 / 15.6; 128 dimensions, one of 1400 17.2 / 16.0, 30 20.9 / 23.6, one of 2000 20.0 / 14.4, 30 26.3 / 31.6; 256 dimensions, 30 of 800 25.1 / 28.0, 8 of 1400 27.6 / 23.6.
@@ -1079,7 +1080,7 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
   const bool dealt = !unit && n_requests <= kDealtRequests && (long)n_requests * each(16) <= 0x3fffffffL / tiles / n_kv_heads;
   // (more than two rounds of units, of several a request, are begun and ended for nothing: 11 requests of up to 238 keys and 155 new tokens, 28 heads, 50 us, on the prompts' kernel 19)
   const bool rounds = unit && each(16) > 1 && all(16) * n_kv_heads > 512;
-  const bool prompt = !(unit || dealt) || rounds || (2 * all(16) - 3 * all(wide)) * n_kv_heads >= (12000 + tiles - 1) / tiles;
+  const bool prompt = !(unit || dealt) || rounds || (2 * all(16) - 5 * all(wide)) * n_kv_heads >= (12000 + tiles - 1) / tiles;
   r.block_cols = prompt ? wide : 16;
   r.col_tiles = (int)each(r.block_cols);
   const long units = n_kv_heads * all(r.block_cols);
@@ -1166,25 +1167,25 @@ extern "C" int mui_paged_attention(mui_stream_t stream, const mui_paged_attentio
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(plan.workgroups ? plan.workgroups : blocks));
   const dim3 join((unsigned)(((long)a.n_rows * a.n_q_heads + 3) / 4));
-#define MUI_PAGED_GO(TT, DC, PIECES)                                                                                                       \
+#define MUI_PAGED_GO(TT, DC)                                                                                                               \
   do {                                                                                                                                     \
     if (prompt) {                                                                                                                          \
-      hipLaunchKernelGGL((paged_tiles_kernel<TT, DC, PIECES, DC == 4 ? 1 : 2>), dim3((unsigned)blocks, plan.splits), dim3(256), 0, s, p); \
+      hipLaunchKernelGGL((paged_tiles_kernel<TT, DC, DC == 4 ? 1 : 2>), dim3((unsigned)blocks, plan.splits), dim3(256), 0, s, p); \
       if (p.part) hipLaunchKernelGGL((paged_join_kernel<TT, DC>), join, dim3(256), 0, s, p);                                               \
     } else {                                                                                                                               \
       if constexpr (DC < 4) {                                                                                                              \
         if (plan.waves == 8)                                                                                                               \
-          hipLaunchKernelGGL((paged_columns_kernel<TT, DC, PIECES, 8>), grid, dim3(512), 0, s, p);                                         \
+          hipLaunchKernelGGL((paged_columns_kernel<TT, DC, 8>), grid, dim3(512), 0, s, p);                                         \
       }                                                                                                                                    \
       if constexpr (DC > 1) {                                                                                                              \
         if (plan.waves == 4)                                                                                                               \
-          hipLaunchKernelGGL((paged_columns_kernel<TT, DC, PIECES, 4>), grid, dim3(256), 0, s, p);                                         \
+          hipLaunchKernelGGL((paged_columns_kernel<TT, DC, 4>), grid, dim3(256), 0, s, p);                                         \
       }                                                                                                                                    \
       if (p.part) hipLaunchKernelGGL((paged_join_units_kernel<TT, DC>), join, dim3(256), 0, s, p, plan.workgroups, plan.waves);            \
     }                                                                                                                                      \
   } while (0)
 #define MUI_PAGED_TYPES(DC) \
-  do { if (a.dtype == MUI_DTYPE_F16) MUI_PAGED_GO(F16, DC, 3); else MUI_PAGED_GO(BF16, DC, 2); } while (0)
+  do { if (a.dtype == MUI_DTYPE_F16) MUI_PAGED_GO(F16, DC); else MUI_PAGED_GO(BF16, DC); } while (0)
   if (a.head_dim == 64) MUI_PAGED_TYPES(1); else if (a.head_dim == 128) MUI_PAGED_TYPES(2); else MUI_PAGED_TYPES(4);
   return launch_status();
 }
