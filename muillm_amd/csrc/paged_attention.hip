@@ -737,7 +737,8 @@ __device__ __forceinline__ void prompt_nans(PromptColumns<DC> (&c)[NT], const ui
 }
 
 // The requests' blocks of PER columns, those first whose last column stands furthest behind (it sees most keys; of 64 requests at a time): the n-th one's request, number and
-// the request's rows. Every wave looks for itself, a request a lane. A block's place is counted in blocks too: the request's tokens times heads, and down from there.
+// the request's rows. Every wave looks for itself, a request a lane. A block's place is counted in blocks too: the request's tokens times heads, and down from there. A request that
+// has more blocks than the host has been told keeps its first ones: the others' are all found among those that were launched.
 template <int PER>
 __device__ __forceinline__ bool nth_block(const PagedAttnParams& p, int n, int& b, int& block, PagedSpan& sp) {
   const int lane = threadIdx.x & 63;
@@ -750,6 +751,11 @@ __device__ __forceinline__ bool nth_block(const PagedAttnParams& p, int n, int& 
       blocks = (s.count * p.group + PER - 1) / PER;
       const long last = s.length * p.group / PER;
       top = last < (1 << 30) ? (int)last : 1 << 30;
+      const int over = blocks - p.col_tiles;
+      if (over > 0) {
+        top -= over;
+        blocks = p.col_tiles;
+      }
     }
     const int here = p.t.n_requests - r0 < kWave ? p.t.n_requests - r0 : kWave;
     int total = 0, high = 0, low = 1 << 30;  // the places there are
@@ -1033,6 +1039,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
   const PagedSpan sp = paged_span(p.t, b);
   if (row < sp.row0 || row >= sp.row0 + sp.count) return;
   const int col = (row - sp.row0) * p.group + head % p.group;
+  if (col / p.block_cols >= p.col_tiles) return;  // (beyond what the host has been told: nobody's work)
   const int n_tiles = column_block(p, sp, col / p.block_cols, p.block_cols).range.count();
   int splits = n_tiles > 0 ? (n_tiles + p.split_tiles - 1) / p.split_tiles : 1;
   splits = splits < p.splits ? splits : p.splits;
