@@ -835,7 +835,7 @@ int mui_channel_delta(mui_stream_t stream, int dtype, const mui_channel_delta_t*
 
 /* The calls' arguments come in structs, whose unused pointers are NULL; out of them nothing is kept.
  *
- * Rotates and appends. q [n_rows, n_q_heads, head_dim] (may be NULL), k, v [n_rows, n_kv_heads, head_dim] with strides in elements (multiples of 8); q_out dense (may be q).
+ * Rotates and appends. q [n_rows, n_q_heads, head_dim] (may be NULL), k, v [n_rows, n_kv_heads, head_dim] with strides in elements (multiples of 8); q_out dense (may be q; not over k or v).
  * The first rot_dim (a multiple of 16) dimensions of q and k turn by the angle position * inv_freq[i] (double [rot_dim / 2]; its whole turns dropped in double precision):
  * pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) if interleaved; cosine and sine times rope_scale. positions: int64 [n_rows], or NULL: a token's place in its request.
  * q_out is rounded once. Per page and head, over the tokens appended: scale = 2^e, e the smallest integer >= -120 with max |x| <= 448 * 2^e (infinities and NaN left

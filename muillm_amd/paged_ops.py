@@ -135,6 +135,16 @@ def _scratch_bytes(*sizes: int) -> int:
     return _lib.load().mui_paged_attention_scratch_bytes(*sizes)
 
 
+def _over(out: torch.Tensor, x: torch.Tensor) -> bool:
+    """Whether the dense `out` has bytes between the first and the last of x [rows, heads, dim]."""
+    rows, heads, dim = x.shape
+    if not (rows and heads and out.numel()):
+        return False
+    begin, size = x.data_ptr(), x.element_size()
+    end = begin + size * ((rows - 1) * x.stride(0) + (heads - 1) * x.stride(1) + dim)
+    return begin < out.data_ptr() + size * out.numel() and out.data_ptr() < end
+
+
 def _output(out: Optional[torch.Tensor], q: torch.Tensor, in_place: bool) -> torch.Tensor:
     if out is None:
         return torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -142,10 +152,7 @@ def _output(out: Optional[torch.Tensor], q: torch.Tensor, in_place: bool) -> tor
         raise RuntimeError("out must be a contiguous tensor of q's shape and type")
     if in_place and out.data_ptr() == q.data_ptr() and q.is_contiguous():
         return out
-    rows, heads, dim = q.shape
-    begin, size = q.data_ptr(), q.element_size()
-    end = begin + size * ((rows - 1) * q.stride(0) + (heads - 1) * q.stride(1) + dim)
-    if out.numel() and begin < out.data_ptr() + size * out.numel() and out.data_ptr() < end:
+    if _over(out, q):
         raise RuntimeError("out must not lie over q" + (", unless it is q" if in_place else ""))
     return out
 
@@ -163,7 +170,8 @@ def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, kv
     A page's scale is the smallest power of two with which its largest value fits 448, and does not fall while earlier tokens stand there; where it
     rises their codes follow. Infinities and NaN become NaN. A page that is appended to belongs to one request. Tokens without a place (a table entry that is no
     page, a length beyond the table) are not written. max_tokens: at least the most new tokens of a request (default: 1 without offsets, else all rows): 1 takes
-    the kernel for single tokens, others' tokens behind the first are then not appended. out may be q itself."""
+    the kernel for single tokens, others' tokens behind the first are then not appended. out may be q itself; it must not
+    lie over k or v."""
     n_rows = k.shape[0]
     n, width, step = _places(kv, table, lengths, offsets, n_rows)
     code, dtype = _dtype(k), k.dtype
@@ -173,7 +181,9 @@ def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, kv
     qp = op = fp = 0
     if q is not None:
         heads, qt, qh = _rows(q, "q", kv, None, dtype, n_rows)
-        out = _output(out, q, True)
+        given, out = out, _output(out, q, True)
+        if given is not None and (_over(out, k) or _over(out, v)):
+            raise RuntimeError("out must not lie over k or v, which the same launch reads")
         qp, op = q.data_ptr(), out.data_ptr()
     rot = 0
     if inv_freq is not None:
