@@ -83,3 +83,25 @@ def test_quiet_pages_beside_loud_ones(lengths, new, dtype, dim, page, apart):
         for i in (1, 4, 6, 7):
             cache.scales[1][int(table[0, i])] = 2.0 ** -8
     hold(dtype, dim, page, lengths, new, 0.0, 2.0 ** -11 if dtype is BF16 and new[0] > 1 else 2.0 ** -22, change=change)
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(F16, 128, 64), (BF16, 128, 64), (BF16, 64, 64), (F16, 256, 64)])
+@pytest.mark.parametrize("lengths,new", [([300, 90], [1, 1]), ([300, 90], [150, 90]), ([2600, 90], [1, 1])], ids=str)
+@pytest.mark.parametrize("power", [-126, -125, -124, -123, -121, 100, 112])
+def test_value_scales_at_the_ends(power, lengths, new, dtype, dim, page):
+    """Any power of two is a scale: fp16 outputs of the smallest are zeros, bf16 ones the same bits as at 1, but for the power."""
+    cache = Cache(2 + sum(-(-n // page) for n in lengths), 2, page, dim, 7)
+    table = make_table(lengths, page, cache.n_pages, 7)
+    q = torch.randn((sum(new), 4, dim), generator=torch.Generator().manual_seed(3)).to(dtype)
+    t, ln, off = gpu(table, torch.tensor(lengths), offsets_of(new))
+    outs = []
+    for e in (0, power):
+        cache.scales[1][:] = 2.0 ** e
+        outs.append(paged_ops.paged_attention(q.to(DEV), cache.to_gpu(), t, ln, off, max_tokens=max(new)).cpu())
+    if dtype is F16:
+        assert bool((outs[1] == 0).all()) if power < 0 else bool(outs[1].isinf().any())
+    else:
+        want = (outs[0].double() * 2.0 ** power).to(dtype)
+        normal = outs[0].double().abs() * 2.0 ** power >= 2.0 ** -126
+        assert float(normal.float().mean()) > 0.5 and torch.equal(outs[1][normal], want[normal])
+        assert bool((outs[1].double()[~normal].abs() <= 2.0 ** -126).all())
