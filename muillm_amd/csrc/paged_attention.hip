@@ -30,7 +30,7 @@ struct PagedAttnParams {
   uint16_t* out;
 };
 
-constexpr float kNoMax = -1e30f;
+constexpr float kNoMax = -0x1.fffffep127f;  // below every score
 constexpr int kDealtRequests = 1024;  // requests whose tiles are dealt out (more give a workgroup each anyway)
 
 // tiles of a workgroup's share, at least one a wave

@@ -105,3 +105,25 @@ def test_value_scales_at_the_ends(power, lengths, new, dtype, dim, page):
         normal = outs[0].double().abs() * 2.0 ** power >= 2.0 ** -126
         assert float(normal.float().mean()) > 0.5 and torch.equal(outs[1][normal], want[normal])
         assert bool((outs[1].double()[~normal].abs() <= 2.0 ** -126).all())
+
+
+@pytest.mark.parametrize("dim,page", [(64, 64), (128, 64), (256, 128)])
+@pytest.mark.parametrize("lengths,new", [([1, 70, 700], [1, 1, 1]), ([40, 70, 300], [40, 30, 300]), ([2600, 3], [1, 1])], ids=str)
+@pytest.mark.parametrize("size", [-1e29, -1e31, -1e35, 1e35])
+def test_scores_at_the_ends_of_32_bits(dim, page, lengths, new, size):
+    """All of a token's scores are the same large number: its keys weigh the same."""
+    cache = Cache(2 + sum(-(-n // page) for n in lengths), 1, page, dim, 8)
+    cache.codes[0][:] = 0.0
+    cache.codes[0][..., 3] = 256.0
+    cache.scales[0][:] = 2.0 ** 40
+    table = make_table(lengths, page, cache.n_pages, 8)
+    q = torch.zeros((sum(new), 2, dim))
+    q[..., 3] = size / 2.0 ** 48
+    q = q.to(BF16)
+    t, ln, off = gpu(table, torch.tensor(lengths), offsets_of(new) if max(new) > 1 else None)
+    got = paged_ops.paged_attention(q.to(DEV), cache.to_gpu(), t, ln, off, scale=1.0).cpu().double()
+    even = cache.clone()
+    even.codes[0][:] = 0.0
+    want, bound = definition(even, torch.zeros_like(q), table, lengths, new, 1.0, 2.0 ** -11)
+    allowed = bound + torch.finfo(BF16).eps / 2 * (want.abs() + bound)
+    assert bool(((got - want).abs() <= allowed).all())
