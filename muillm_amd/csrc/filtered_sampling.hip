@@ -288,7 +288,7 @@ __device__ __forceinline__ void sample_token(const SampleParams& p, SampleShared
       }
       if (n < kept) kept = n;
     }
-    if (kept < 1) kept = 1;
+    if (kept < 1 || min_p > 1.f) kept = 1;  // (no weight reaches a min_p above 1)
     double all = weight_of_first(kept);
     if (min_p > 0.f && kept > 1) {  // (weights and logits fall together)
       const double least = log((double)min_p);
