@@ -183,10 +183,9 @@ __device__ __forceinline__ void times_here(f32x4& x, float f) {
   x = f32x4{a, b, c, d};
 }
 
-// What a tile's score products are multiplied by. Not 0, which a query and keys of zeros would make it (2^-120 is a page's scale then): a hidden key's score is -inf. Nor more
-// than leaves the largest products finite (256 of 2^8 times 448, of fp16 2^16 times 448).
-template <typename T>
-__device__ __forceinline__ float score_unit(float query, float keys) { return __builtin_amdgcn_fmed3f(query * keys, 0x1p-126f, T::kDtype == MUI_DTYPE_F16 ? 0x1p94f : 0x1p100f); }
+// What a tile's score products are multiplied by. Not 0, which a query and keys of zeros would make it (2^-120 is a page's scale then): a hidden key's score is -inf. Nor
+// infinite, which products of 0 would make NaN.
+__device__ __forceinline__ float score_unit(float query, float keys) { return __builtin_amdgcn_fmed3f(query * keys, 0x1p-126f, -kNoMax); }
 
 // Scores so far from zero that what a fused product keeps and a maximum has rounded away counts in an exponential: they are rounded first.
 __device__ __forceinline__ bool is_far(float most) { return fabsf(most) >= 0x1p22f && most > kNoMax; }
@@ -229,7 +228,7 @@ __device__ __forceinline__ void attend_tile(Columns<DC>& c, const QueryTile<DC>&
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[i][r] = seen >> (4 * i + r) & 1u ? s[i][r] : -INFINITY;
   }
-  float unit = score_unit<T>(q.unit, ks);
+  float unit = score_unit(q.unit, ks);
   float most = s[0][0];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -948,7 +947,7 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
     prompt_most<NT>(most, s);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      unit[n] = score_unit<T>(q[n].unit, at.ks);
+      unit[n] = score_unit(q[n].unit, at.ks);
       most[n] *= unit[n];
     }
     prompt_move<DC, NT>(c, most, s, unit);
@@ -986,7 +985,7 @@ __global__ void __launch_bounds__(256, DC == 4 ? 1 : 2) paged_tiles_kernel(const
     prompt_most<NT>(most, s);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      unit[n] = score_unit<T>(q[n].unit, at1.ks);
+      unit[n] = score_unit(q[n].unit, at1.ks);
       most[n] *= unit[n];
     }
     if (kWhole || page1 >= 0) put_values(at1, slot ^ 1, i + 1, whole);

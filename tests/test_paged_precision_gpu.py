@@ -127,3 +127,22 @@ def test_scores_at_the_ends_of_32_bits(dim, page, lengths, new, size):
     want, bound = definition(even, torch.zeros_like(q), table, lengths, new, 1.0, 2.0 ** -11)
     allowed = bound + torch.finfo(BF16).eps / 2 * (want.abs() + bound)
     assert bool(((got - want).abs() <= allowed).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lengths,new", [([128], [1]), ([2624], [1]), ([128], [64]), ([2624], [64])], ids=str)
+def test_very_large_scores_of_pages_of_different_scales(dim, lengths, new):
+    """2^111 beside 2^110: the larger one has all the weight, whatever the pages' scales are."""
+    cache = Cache(lengths[0] // 64 + 2, 1, 64, dim, 9)
+    cache.codes[0][:] = 0.0
+    table = make_table(lengths, 64, cache.n_pages, 9)
+    first, second = int(table[0, 0]), int(table[0, 1])
+    cache.scales[0][:] = 2.0 ** 46
+    cache.scales[0][first], cache.codes[0][first, :, 7, 3] = 2.0 ** 50, 2.0
+    cache.codes[0][second, :, 5, 3] = 16.0
+    q = torch.zeros((sum(new), 2, dim))
+    q[..., 3] = 2.0 ** 60
+    t, ln, off = gpu(table, torch.tensor(lengths), offsets_of(new) if max(new) > 1 else None)
+    got = paged_ops.paged_attention(q.to(BF16).to(DEV), cache.to_gpu(), t, ln, off, scale=1.0).cpu().double()
+    want = cache.values(1, table[0].long(), lengths[0])[0, 7]
+    assert bool(((got - want).abs() <= torch.finfo(BF16).eps / 2 * want.abs() * (1 + 2.0 ** -10)).all())
