@@ -825,7 +825,7 @@ int mui_channel_delta(mui_stream_t stream, int dtype, const mui_channel_delta_t*
  *
  * The cache of one layer: pages of page_tokens (64, 128 or 256) tokens. k_pages: e4m3 codes [n_pages, n_kv_heads, page_tokens / 64, head_dim / 64, 64, 64], the last
  * two token and dimension. v_pages: e4m3 codes [n_pages, n_kv_heads, page_tokens / 64, head_dim, 4, 4, 4], the last three g, t, i of token 16 t + 4 g + i of the 64.
- * k_scale, v_scale: fp32 [n_pages, n_kv_heads], powers of two; a value is code * scale. head_dim 64, 128 or 256; pages, rows and outputs 16-byte aligned.
+ * k_scale, v_scale: fp32 [n_pages, n_kv_heads], powers of two (2^-126 and more); a value is code * scale. head_dim 64, 128 or 256; pages, rows and outputs 16-byte aligned.
  * table: int32 [n_requests, table_pages], rows table_stride apart: a request's pages in order (fewer than 2^31 tokens of them). lengths: int64 [n_requests], a request's tokens, the call's
  * among them. offsets: int64 [n_requests + 1]: a request's new tokens are the rows offsets[b] .. offsets[b + 1] - 1 of the call's n_rows; NULL: row b (n_rows ==
  * n_requests). All of it on the device and read there. Whatever it holds, nothing outside the given buffers is read or written: an entry that is no page and places
@@ -840,7 +840,7 @@ int mui_channel_delta(mui_stream_t stream, int dtype, const mui_channel_delta_t*
  * pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) if interleaved; cosine and sine times rope_scale. positions: int64 [n_rows], or NULL: a token's place in its request.
  * q_out is rounded once. Per page and head, over the tokens appended: scale = 2^e, e the smallest integer >= -120 with max |x| <= 448 * 2^e (infinities and NaN left
  * out), at least the scale that stands there if the page holds earlier tokens, whose codes are then multiplied by the quotient and rounded again; code = x / scale,
- * nearest even; infinities and NaN give NaN codes. A page that is appended to must belong to one request. Rows behind the last request are left as they are.
+ * nearest even; infinities and NaN give NaN codes. A page that is appended to must belong to one request and stand in its row once. Rows behind the last request are left as they are.
  * max_tokens 1: only the first new token of a request is appended; any other number: all of them. */
 typedef struct mui_paged_append_args {
   const void* q;
@@ -864,7 +864,7 @@ int mui_paged_append(mui_stream_t stream, const mui_paged_append_args_t* args);
 
 /* Causal attention of q [n_rows, n_q_heads, head_dim] over the cache, which holds the new tokens already: out (dense) = softmax(scale * q . k) v over the keys at positions
  * s <= p, p that of the token, and s > p - window or s < keep_first if window > 0. n_q_heads a multiple of n_kv_heads, scale > 0. A token without a key gives
- * zeros. Keys that a token does not see do not touch it, whatever their codes are. out must not lie over q. scratch: mui_paged_attention_scratch_bytes() bytes for
+ * zeros. Keys that a token does not see do not touch it, whatever their codes are. Scores, their sums and the values' are 32 bits. At most 65535 requests. out must not lie over q. scratch: mui_paged_attention_scratch_bytes() bytes for
  * max_length cut to table_pages * page_tokens, 16-byte aligned (NULL if 0). */
 typedef struct mui_paged_attention_args {
   const void* q;
@@ -886,7 +886,7 @@ size_t mui_paged_attention_scratch_bytes(int n_rows, int n_requests, int max_tok
                                          int head_dim);
 int mui_paged_attention(mui_stream_t stream, const mui_paged_attention_args_t* args);
 
-/* Per row of 16-bit logits [rows, vocab]: a token from random_numbers[row], uniform in [0, 1). w_i = exp((l_i - max l) / temperature) in double precision; tokens in order of
+/* Per row of 16-bit logits [rows, vocab] (at most 65535 rows): a token from random_numbers[row], uniform in [0, 1). w_i = exp((l_i - max l) / temperature) in double precision; tokens in order of
  * falling logits, equal ones by rising index. Kept are the first top_k (<= 0: all); of those the ones in front of which less than top_p (>= 1: all) times the
  * top_k's weight lies; of those the ones with w >= min_p; the first one always. out_token = the first whose cumulative weight exceeds random_numbers[row] times
  * the kept weight, out_probability (may be NULL) its share of it. temperature <= 0: the largest logit. NaN and -inf are never drawn; a row of nothing else gives token 0

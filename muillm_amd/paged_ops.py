@@ -168,7 +168,7 @@ def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, kv
     are the tokens' own unless positions (int64 [rows]) says otherwise.
 
     A page's scale is the smallest power of two with which its largest value fits 448, and does not fall while earlier tokens stand there; where it
-    rises their codes follow. Infinities and NaN become NaN. A page that is appended to belongs to one request. Tokens without a place (a table entry that is no
+    rises their codes follow. Infinities and NaN become NaN. A page that is appended to belongs to one request and stands in its row once. Tokens without a place (a table entry that is no
     page, a length beyond the table) are not written. max_tokens: at least the most new tokens of a request (default: 1 without offsets, else all rows): 1 takes
     the kernel for single tokens, others' tokens behind the first are then not appended. out may be q itself; it must not
     lie over k or v."""
