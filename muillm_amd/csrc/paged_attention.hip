@@ -1079,13 +1079,16 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
   // The kernel for single tokens takes 2.2 ns for a block of 16 columns and a tile, the one for prompts 5 to 6 for a block of 128, and 6 us more to begin with and to join. us, the one / the
   // other, 32 heads, 8 KV heads, 128 bf16 dimensions: one request of 1000 keys and 32 new tokens 12 / 26; of 8000 and 16 24 / 31, 32 33 / 32; 16 requests of 1000 and 16 23 / 34, 32 42 / 39;
   // of 8000 and 4 54 / 92, 8 93 / 96 (fp16 93 / 114, 64 dimensions 41 / 74, 256 138 / 179), 32 281 / 119.
-  const bool sparse = (long)n_requests * each(16) > 2 * all(16);  // a workgroup per unit would find most of them empty: those that begin and end take 8 ns each
   // A workgroup per unit needs no scan and no joining launch. us, a unit each / dealt out, 8 KV heads, requests of equal lengths, which suit it best: 64 dimensions, 8 requests of 1400 keys
-  // 12.3 / 15.6; 128 dimensions, one of 1400 17.2 / 16.0, 30 20.9 / 23.6, one of 2000 20.0 / 14.4, 30 26.3 / 31.6; 256 dimensions, 30 of 800 25.1 / 28.0, 8 of 1400 27.6 / 23.6.
+  // 10.6 / 13.6; 128 dimensions, one of 1400 13.4 / 14.7, 30 17.9 / 22.0, one of 2000 15.6 / 12.1, 30 23.7 / 30.7; 256 dimensions, 30 of 800 25.7 / 28.2, 8 of 1400 29.4 / 22.6.
+  // Workgroups without work take 8 ns each: a thousand of them are as long as dealing out (16 requests of up to 60 new tokens, 764 of 1728 workgroups with work, 25 / 30).
+  const bool sparse = ((long)n_requests * each(16) - all(16)) * n_kv_heads > 1024;
   const bool unit = !sparse && (tiles <= (head_dim == 256 ? 16 : 24) || n_requests > kDealtRequests);
   const bool dealt = !unit && n_requests <= kDealtRequests && (long)n_requests * each(16) <= 0x3fffffffL / tiles / n_kv_heads;
-  // (more than two rounds of units, of several a request, are begun and ended for nothing: 11 requests of up to 238 keys and 155 new tokens, 28 heads, 50 us, on the prompts' kernel 19)
-  const bool rounds = unit && each(16) > 1 && all(16) * n_kv_heads > 512;
+  // Units of short caches, several a request, go to the prompts' kernel from the third round of them on (dealt out: the second) where they fill its blocks. us, units / there: 4 KV heads of
+  // 128 dimensions, 28 heads, 64 requests of 200 keys and 20 new tokens (4.5 units to a block) 57 / 31, 200 and up to 8 (2.9) 75 / 58, 200 and up to 3 (1.9) 41 / 57; 8 and 32, 200 of 1500
+  // and 8 (2) 198 / 314; 11 requests of up to 238 keys and 155 new tokens, 28 heads, dealt out 47 / 19.
+  const bool rounds = each(16) > 1 && tiles <= 24 && all(16) * n_kv_heads > (unit ? 512 : 256) && 2 * all(16) > 5 * all(wide);
   const bool prompt = !(unit || dealt) || rounds || (2 * all(16) - 5 * all(wide)) * n_kv_heads >= (12000 + tiles - 1) / tiles;
   r.block_cols = prompt ? wide : 16;
   r.col_tiles = (int)each(r.block_cols);
@@ -1112,9 +1115,9 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
     return r;
   }
   // Eight waves to a workgroup and one workgroup to a CU, or four and two: eight cut fewer units, four have more of them at work where the shares are small. us, four / eight:
-  // 64 heads x 64 dimensions, 16 requests of 4096 keys 27.7 / 22.0; 128 dimensions, 32 requests of 200 to 4096 keys 35.5 / 40.7, 64 of 4096 to 16384 195.6 / 190.7.
-  // 256 dimensions: a wave's registers are all of a SIMD's.
-  r.waves = head_dim == 256 ? 4 : head_dim == 64 || unit || units * tiles >= 128 * 256 ? 8 : 4;
+  // 64 heads x 64 dimensions, 16 requests of 4096 keys 27.7 / 22.0; 8 KV heads of 128 dimensions, 32 requests of 200 to 4096 keys 44 / 53, 64 76 / 98, 100 of 2000 79 / 77, 128 of 500 to
+  // 8000 194 / 196, 16 of 30000 160 / 156, 64 of 4096 to 16384 223 / 219. 256 dimensions: a wave's registers are all of a SIMD's.
+  r.waves = head_dim == 256 ? 4 : head_dim == 64 || unit || units * tiles >= 192 * 256 ? 8 : 4;
   if (unit) return r;
   const long wanted = (units * tiles + r.waves - 1) / r.waves, most = head_dim == 256 || r.waves == 8 ? 256 : 512;
   r.workgroups = (int)(wanted < most ? wanted : most);

@@ -11,8 +11,10 @@ pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
 
 BEYOND = [  # requests' lengths and new tokens, max_tokens, heads, KV heads
-    ([100 + 7 * i for i in range(40)], [8] * 17 + [64] + [8] * 22, 8, 32, 8),                  # short caches, a block of columns each
-    ([90 + i for i in range(100)], [8] * 99 + [90], 8, 16, 4),                                 # more requests than a wave has lanes
+    ([100 + 7 * i for i in range(40)], [8] * 17 + [64] + [8] * 22, 8, 32, 8),                  # short caches, a workgroup a unit
+    ([90 + i for i in range(100)], [8] * 99 + [90], 8, 16, 4),
+    ([100 + 7 * i for i in range(40)], [30] * 17 + [90] + [30] * 22, 30, 16, 4),               # prompts, a block of columns each
+    ([90 + i for i in range(100)], [20] * 99 + [90], 20, 8, 2),                                # more requests than a wave has lanes
     ([9000, 9100, 12800], [32, 100, 32], 32, 8, 2),                                            # keys divided and joined
     ([9000, 9100, 12800], [4, 40, 4], 4, 8, 2),                                                # dealt out and joined
     ([100, 200, 150], [2, 30, 2], 2, 8, 2),                                                    # a workgroup a unit
