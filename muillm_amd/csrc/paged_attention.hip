@@ -370,8 +370,8 @@ __device__ __forceinline__ PagedSpan span_of_lane(const PagedSpan& s, int l) {
 // equal shares, whatever the requests' lengths: the units that a share cuts are joined by a second launch. (Short caches: a workgroup per unit, nothing to join.) The waves of
 // a workgroup take every W-th tile each and meet in LDS. Two waves on a SIMD keep the memory busy, 16 KB on the way for each (128 dimensions): with the next tile requested
 // while one is worked on as well their registers do not suffice (64 requests of 4096 to 16384 tokens 204 instead of 187 us).
-// The cache's bytes bound it where there are many: those 64 requests, 8 KV heads of 128 dimensions (1.17 GB), 187 us, 6.2 TB/s; 32 requests of 200 to 4096 (90 MB) 29.6. With few it is the loads that
-// wait for one another (length, page, keys and values, again for each tile of a wave): 700 keys 9.4 us.
+// The cache's bytes bound it where there are many: those 64 requests, 8 KV heads of 128 dimensions (1.17 GB), 186 us, 6.2 TB/s; 32 requests of 200 to 4096 (90 MB) 27.8. With few it is the loads that
+// wait for one another (length, page, keys and values, again for each tile of a wave): 700 keys 9.0 us.
 template <typename T, int DC, int W>
 __global__ void __launch_bounds__(64 * W, DC == 4 ? W / 4 : 2) paged_columns_kernel(const PagedAttnParams p) {
   constexpr int D = DC * 64, kThreads = 64 * W;
@@ -1097,9 +1097,9 @@ static PagedPlan paged_plan(int n_rows, int n_requests, int max_tokens, int max_
   r.splits = 1;
   r.split_tiles = (int)tiles;
   if (prompt) {
-    // Keys divided among the workgroups that the card has room for at once, 8 tiles each at least, where that ends earlier: a workgroup takes 1.4 us a tile, two on a CU 2.2 (256 dimensions,
-    // one on a CU: 2.5), joining 10. us undivided / divided: 1000 tokens of one request 30 / 42 (two parts), 100 of 4 requests of 8000 keys 104 (two) / 82 (four), two of 1477, one KV head,
-    // 51 / 43 (two); 256 dimensions, 500 behind 1000 49 / 67 (more than there is room for), 64 behind 8000 59 / 45.
+    // Keys divided among the workgroups that the card has room for at once, 8 tiles each at least, where that ends earlier: a workgroup takes 1.4 us a tile, two on a CU 2.2 (256
+    // dimensions, one on a CU: 2.5), joining 10. us undivided / in two / in four: 1000 tokens of one request 39 / 47 / 52, 100 of 4 requests of 8000 keys 228 / 134 / 99, two of 1477,
+    // 4 heads on one, 51 / 41 / 36; 256 dimensions, 500 behind 1000 61 / 80 / 97 (more than there is room for), 64 behind 8000 260 / 145 / 85 (in eight 54).
     const long room = head_dim == 256 ? 256 : 512;
     long splits = 1, least = 0;
     for (long n = 1; n == 1 || (n <= tiles / 8 && n * units <= room); n += 1 + n / 16) {
